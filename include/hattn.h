@@ -651,6 +651,117 @@ int hattn_gated_rmsnorm_bwd(const void* y, const void* z, long long ldz, const v
                             int dtype_z, int dtype_w, int dtype_dout, int dtype_dy,
                             int dtype_dz, void* ws, size_t ws_bytes, void* stream);
 
+/*
+ * Mixers and norm of a hybrid stack, next to the log-linear scans.  No counterpart in
+ * the reference.  Invalid sizes are HATTN_ERR_VALUE, sizes and types outside what is
+ * built HATTN_ERR_NOT_IMPLEMENTED.
+ */
+
+/*
+ * Layer norm over rows of n elements, with the residual stream's addition in front:
+ *   s = round(x + residual) (residual NULL: s = x, nothing written),
+ *   y = (s - mean(s)) rstd weight + bias,  rstd = (mean((s - mean(s))^2) + eps)^-1/2
+ * x, y [rows, n] in dtype_x; residual, s [rows, n] in dtype_r (dtype_x or FP32);
+ * weight, bias [n] in dtype_w, either may be NULL; mean, rstd [rows] fp32 for the
+ * backward, both or neither NULL.  n <= 16384.
+ */
+int hattn_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                         void* y, void* s, float* mean, float* rstd, long long rows, int n,
+                         float eps, int dtype_x, int dtype_r, int dtype_w, void* stream);
+
+/*
+ * Backward of the layer norm: dy in dtype_x; ds (may be NULL) the gradient that reaches
+ * s past the norm, in s's dtype_s.  dx (dtype_x) and dresidual (dtype_s) receive the same
+ * gradient, each may be NULL; dweight, dbias [n] in dtype_w, each may be NULL, summed in
+ * a fixed order.  Workspace: hattn_layer_norm_bwd_workspace(rows, n) bytes where dweight
+ * or dbias is given.
+ */
+size_t hattn_layer_norm_bwd_workspace(long long rows, int n);
+int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, const float* rstd,
+                         const void* dy, const void* ds, void* dx, void* dresidual, void* dweight,
+                         void* dbias, long long rows, int n, int dtype_x, int dtype_s, int dtype_w,
+                         void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Gated linear recurrence, per channel: h_t = exp(g_t) h_{t-1} + x_t, o_t = h_t.
+ * x, o [B, T, D] in dtype_x; g [B, T, D] in dtype_g (dtype_x or FP32); h0, ht [B, D] fp32
+ * state before and after, each may be NULL (h0: zero); lengths [B] int32 or NULL: row b
+ * has lengths[b] tokens (clamped to [0, T]), its later outputs are zero, its later inputs
+ * are not used, and ht is the state after its last token.  carry
+ * [B, hattn_gated_recurrence_segments(T), D] fp32 (NULL: not kept) is what the backward
+ * takes.  Workspace, forward and backward: hattn_gated_recurrence_workspace(B, T, D)
+ * bytes, 8-byte aligned, contents on entry ignored.
+ *
+ * Workgroups wait, with a bounded poll, for the states of earlier segments; a wait that
+ * gives up (two calls that overlap on one workspace) gives NaN, not plausible numbers.
+ */
+int hattn_gated_recurrence_segments(int T);
+size_t hattn_gated_recurrence_workspace(int B, int T, int D);
+int hattn_gated_recurrence_fwd(const void* x, const void* g, const float* h0, const int* lengths,
+                               void* o, float* ht, float* carry, int B, int T, int D, int dtype_x,
+                               int dtype_g, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Its backward: dout [B, T, D] in dtype_x, dht [B, D] fp32 (may be NULL) the gradients of
+ * o and ht; dx in dtype_x, dg in dtype_g (zero past a row's length), dh0 [B, D] fp32 (may
+ * be NULL).  carry from the forward of the same inputs.
+ */
+int hattn_gated_recurrence_bwd(const void* x, const void* g, const float* carry,
+                               const int* lengths, const void* dout, const float* dht, void* dx,
+                               void* dg, float* dh0, int B, int T, int D, int dtype_x, int dtype_g,
+                               void* ws, size_t ws_bytes, void* stream);
+
+/* One token: state [B, D] fp32 <- exp(g) state + x in place, o = state.  x, g, o [B, D]. */
+int hattn_gated_recurrence_step(float* state, const void* x, const void* g, void* o, int B, int D,
+                                int dtype_x, int dtype_g, void* stream);
+
+/*
+ * Sliding-window attention with sinks: query t sees key s where s <= t and
+ * (t - s < window or s < sinks); o = softmax(scale q k^T) v over the keys it sees.
+ * q [B, T, H, D], k, v [B, T, G, D] with G dividing H (head h reads group h / (H / G)), in
+ * BF16 or FP16; strides: batch, token and head strides of q, then k, then v, in elements,
+ * each a multiple of 8 (the last dimension is contiguous); o [B, T, H, D] contiguous;
+ * lse [B, H, T] fp32 (may be NULL) is what the backward takes.  lengths [B] int32 or NULL:
+ * row b has lengths[b] tokens (clamped to [0, T]); its later outputs are zero and its
+ * later inputs are not read.  D a multiple of 8 up to 128, sinks <= 64, scale > 0; q, k, v
+ * and o aligned to 16 bytes.  An infinity or NaN in k or v of a token that a query does
+ * not see may still reach that query where both fall into one tile of 64 keys.
+ */
+int hattn_sliding_fwd(const void* q, const void* k, const void* v, const int* lengths,
+                      const long long* strides, void* o, float* lse, int B, int T, int H, int G,
+                      int D, int window, int sinks, float scale, int dtype, void* stream);
+
+/*
+ * Its backward: o and lse of the forward, dout [B, T, H, D] contiguous; dq [B, T, H, D],
+ * dk, dv [B, T, G, D] contiguous, summed in a fixed order, zero past a row's length.
+ * Workspace: hattn_sliding_bwd_workspace(..) bytes, aligned to 16.
+ */
+size_t hattn_sliding_bwd_workspace(int B, int T, int H, int G, int D, int window, int sinks);
+int hattn_sliding_bwd(const void* q, const void* k, const void* v, const int* lengths,
+                      const long long* strides, const void* o, const float* lse, const void* dout,
+                      void* dq, void* dk, void* dv, int B, int T, int H, int G, int D, int window,
+                      int sinks, float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * The cache of a decoding batch, k_cache, v_cache [B, G, sinks + window, D] and counts [B]
+ * int32 (tokens seen): slot s < sinks holds token s, slot sinks + i the last token p >=
+ * sinks with p - sinks = i modulo window.
+ *
+ * cache_fill writes the whole cache from prompts k, v [B, T, G, D] (strides: batch, token,
+ * head of k, then v); slots that no token fills are zero, counts[b] = lengths[b] (or T).
+ * step appends one token per row (q [B, H, D], k, v [B, G, D], contiguous) and gives its
+ * attention o [B, H, D]; the counts advance on the device, so that a captured step can be
+ * replayed.  Workspace: hattn_sliding_step_workspace(..) bytes, aligned to 16.
+ */
+int hattn_sliding_cache_fill(const void* k, const void* v, const int* lengths,
+                             const long long* strides, void* k_cache, void* v_cache, int* counts,
+                             int B, int T, int G, int D, int window, int sinks, int dtype,
+                             void* stream);
+size_t hattn_sliding_step_workspace(int B, int H, int G, int D, int window, int sinks);
+int hattn_sliding_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                       int* counts, void* o, int B, int H, int G, int D, int window, int sinks,
+                       float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

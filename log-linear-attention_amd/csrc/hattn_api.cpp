@@ -12,8 +12,8 @@
 #include <cstring>
 #include <initializer_list>
 
+#include "api_common.h"
 #include "hstate.h"
-#include "../../include/hattn.h"
 
 hipError_t hattn_mamba2_fwd_launch(const void* q, const void* k, const void* v, const float* g,
                                    const void* l, void* o, float* gcum, float* ht, void* ws,
@@ -143,7 +143,7 @@ hipError_t hattn_gated_rmsnorm_bwd_launch(const void* y, const void* z, long ldz
                                           int fy, int fz, int fw, int fdo, int fdy, int fdz,
                                           hipStream_t stream);
 
-namespace {
+namespace hattn_api {
 
 thread_local char g_err[512] = {0};
 
@@ -160,16 +160,22 @@ int ok() {
   return HATTN_OK;
 }
 
+int check_hip(hipError_t e, const char* what) {
+  if (e != hipSuccess) return fail(HATTN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+  return ok();
+}
+
+}  // namespace hattn_api
+
+namespace {
+
+using namespace hattn_api;
+
 // ceil(log2(n)) for n >= 1 (ceil_log(NT, 2), base.py:29-30; exact for integers)
 int ceil_log2(int n) {
   int e = 0;
   while ((1 << e) < n) ++e;
   return e;
-}
-
-int check_hip(hipError_t e, const char* what) {
-  if (e != hipSuccess) return fail(HATTN_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-  return ok();
 }
 
 size_t elem_bytes(int code) { return code == HATTN_FP32 ? 4 : 2; }

@@ -1,0 +1,123 @@
+// Layer norm forward with the residual stream's addition:
+//   s = round(x + residual),  mean = sum s / n,  rstd = (sum (s - mean)^2 / n + eps)^-1/2,
+//   y = (s - mean) rstd weight + bias.
+// The row stays in registers between the two sums (the centred second sum keeps
+// what E[s^2] - mean^2 would lose), so every element is read once and written
+// once: bound by the bytes.
+#include "layer_norm_device.h"
+
+namespace hattn {
+
+template <typename TX, typename TR, bool RES, int VEC, int NW, int CH>
+__global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
+    const TX* __restrict__ x, const TR* __restrict__ res, const void* __restrict__ weight,
+    const void* __restrict__ bias, TX* __restrict__ y, TR* __restrict__ s_out,
+    float* __restrict__ mean_out, float* __restrict__ rstd_out, long rows, int n, float eps,
+    int dtype_w) {
+  __shared__ float red[2][NW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int RPB = 4 / NW;  // rows of a workgroup
+  const int first = (NW == 1 ? lane : (int)threadIdx.x) * VEC;
+  constexpr int STEP = 64 * NW * VEC;
+  float w[CH][VEC], b[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int at = first + c * STEP + i;
+      w[c][i] = weight && at < n ? load_param(weight, dtype_w, at) : 1.f;
+      b[c][i] = bias && at < n ? load_param(bias, dtype_w, at) : 0.f;
+    }
+  const float inv_n = 1.f / (float)n;
+  for (long row = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); row < rows;
+       row += (long)gridDim.x * RPB) {
+    const long base = row * n;
+    float v[CH][VEC], sum[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = first + c * STEP;
+      if (at < n) {
+        load_row<TX, VEC>(x + base + at, v[c]);
+        if constexpr (RES) {
+          float r[VEC];
+          load_row<TR, VEC>(res + base + at, r);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[c][i] = to_f32<TR>(from_f32<TR>(v[c][i] + r[i]));
+          store_row<TR, VEC>(s_out + base + at, v[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[0] += v[c][i];
+      }
+    }
+    row_sums<NW>(sum, red[0]);
+    const float mean = sum[0] * inv_n;
+    float sq[1] = {0.f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (first + c * STEP < n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          v[c][i] -= mean;
+          sq[0] += v[c][i] * v[c][i];
+        }
+    row_sums<NW>(sq, red[1]);
+    const float rstd = 1.f / sqrtf(sq[0] * inv_n + eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = first + c * STEP;
+      if (at < n) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = v[c][i] * rstd * w[c][i] + b[c][i];
+        store_row<TX, VEC>(y + base + at, o);
+      }
+    }
+    if (mean_out && (NW == 1 ? lane : (int)threadIdx.x) == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <typename TX, typename TR, bool RES>
+static hipError_t launch_fwd(const void* x, const void* res, const void* weight, const void* bias,
+                             void* y, void* s, float* mean, float* rstd, long rows, int n,
+                             float eps, int dtype_w, hipStream_t stream) {
+  const uintptr_t bits = (uintptr_t)x | (uintptr_t)res | (uintptr_t)y | (uintptr_t)s;
+  const NormShape sh = norm_shape(rows, n, n % 8 == 0 && bits % 16 == 0);
+  const long rpb = 4 / sh.nw;
+  const long want = (rows + rpb - 1) / rpb;
+  const dim3 grid((unsigned)(want < 4096 ? want : 4096));
+#define CALL(VEC, NW, CH)                                                                      \
+  hipLaunchKernelGGL((layer_norm_fwd_kernel<TX, TR, RES, VEC, NW, CH>), grid, dim3(256), 0,    \
+                     stream, (const TX*)x, (const TR*)res, weight, bias, (TX*)y, (TR*)s, mean, \
+                     rstd, rows, n, eps, dtype_w)
+  HATTN_NORM_DISPATCH(sh, CALL);
+#undef CALL
+  return hipGetLastError();
+}
+
+}  // namespace hattn
+
+hipError_t hattn_layer_norm_fwd_launch(const void* x, const void* residual, const void* weight,
+                                       const void* bias, void* y, void* s, float* mean,
+                                       float* rstd, long rows, int n, float eps, int dtype_x,
+                                       int dtype_r, int dtype_w, hipStream_t stream) {
+  using namespace hattn;
+#define GO(TX, TR, RES)                                                                        \
+  return launch_fwd<TX, TR, RES>(x, residual, weight, bias, y, s, mean, rstd, rows, n, eps,    \
+                                 dtype_w, stream)
+  if (!residual) {
+    if (dtype_x == 0) GO(__bf16, __bf16, false);
+    if (dtype_x == 1) GO(_Float16, _Float16, false);
+    GO(float, float, false);
+  }
+  if (dtype_r == 2) {
+    if (dtype_x == 0) GO(__bf16, float, true);
+    if (dtype_x == 1) GO(_Float16, float, true);
+    GO(float, float, true);
+  }
+  if (dtype_x == 0) GO(__bf16, __bf16, true);
+  GO(_Float16, _Float16, true);
+#undef GO
+}

@@ -1,0 +1,304 @@
+// C-ABI entry points of the hybrid stack's mixers and norm (declared in
+// include/hattn.h): layer norm, gated linear recurrence, sliding-window attention.
+// All checks are made here, on the host; the kernels assume what they establish.
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <initializer_list>
+
+#include "api_common.h"
+#include "layer_norm.h"
+#include "recurrence.h"
+#include "sliding.h"
+#include "sliding_step.h"
+
+using namespace hattn_api;
+
+namespace {
+
+const float kLog2e = 1.4426950408889634f;
+
+int check_dtype(int code, const char* what) {
+  if (code < HATTN_BF16 || code > HATTN_FP32)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "%s: dtype code %d", what, code);
+  return HATTN_OK;
+}
+
+bool aligned(std::initializer_list<const void*> ps, size_t n) {
+  uintptr_t bits = 0;
+  for (const void* p : ps) bits |= (uintptr_t)p;
+  return bits % n == 0;
+}
+
+int norm_checks(long long rows, int n, int dtype_x, int dtype_r, int dtype_w, bool residual) {
+  if (rows <= 0 || n <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
+  if (n > kLayerNormMaxN)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "n=%d above %d", n, kLayerNormMaxN);
+  if (int st = check_dtype(dtype_x, "x")) return st;
+  if (int st = check_dtype(dtype_w, "weight")) return st;
+  if (residual && dtype_r != dtype_x && dtype_r != HATTN_FP32)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "residual of dtype code %d with x of %d", dtype_r, dtype_x);
+  return HATTN_OK;
+}
+
+int recurrence_checks(int B, int T, int D, int dtype_x, int dtype_g) {
+  if (B <= 0 || T <= 0 || D <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
+  if (int st = check_dtype(dtype_x, "x")) return st;
+  if (dtype_g != dtype_x && dtype_g != HATTN_FP32)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "g of dtype code %d with x of %d", dtype_g, dtype_x);
+  const long long strips = (D + 63) / 64;
+  if (B * strips * hattn_recurrence_segments(T) >= (1LL << 31))
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d D=%d: 2^31 segments", B, T, D);
+  return HATTN_OK;
+}
+
+size_t recurrence_ws(int B, int T, int D) {
+  const size_t nseg = hattn_recurrence_segments(T);
+  return nseg > 1 ? nseg * B * ((D + 63) / 64) * 64 * 8 : 0;
+}
+
+int sliding_checks(int B, int H, int G, int D, int window, int sinks, float scale, int dtype) {
+  if (B <= 0 || H <= 0 || G <= 0 || D <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
+  if (H % G != 0) return fail(HATTN_ERR_VALUE, "H=%d is not a multiple of G=%d", H, G);
+  if (window < 1) return fail(HATTN_ERR_VALUE, "window=%d below 1", window);
+  if (sinks < 0) return fail(HATTN_ERR_VALUE, "sinks=%d below 0", sinks);
+  if (!(scale > 0.f) || !(scale <= 1e30f)) return fail(HATTN_ERR_VALUE, "scale must be positive and finite");
+  if (sinks > kMaxSinks)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "sinks=%d above %d", sinks, kMaxSinks);
+  if (D % 8 != 0 || D > 128)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "D=%d is not a multiple of 8 up to 128", D);
+  if (dtype != HATTN_BF16 && dtype != HATTN_FP16)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "dtype code %d (bf16 or fp16 only)", dtype);
+  return HATTN_OK;
+}
+
+// Strides in elements, batch / token / head of q, k, v: 16-byte rows.
+int stride_checks(const long long* st, int n) {
+  for (int i = 0; i < n; ++i)
+    if (st[i] % 8 != 0)
+      return fail(HATTN_ERR_VALUE, "stride %lld is not a multiple of 8 elements", st[i]);
+  return HATTN_OK;
+}
+
+int sliding_fill(SlidingArgs& p, const void* q, const void* k, const void* v, const int* lengths,
+                 const long long* strides, int B, int T, int H, int G, int D, int window, int sinks,
+                 float scale, int dtype) {
+  if (T <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
+  if (int st = sliding_checks(B, H, G, D, window, sinks, scale, dtype)) return st;
+  if (!q || !k || !v || !strides) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (int st = stride_checks(strides, 9)) return st;
+  if ((long long)B * H * ((T + 127) / 128) >= (1LL << 31) - 8 || T > INT_MAX / 2)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: too many blocks", B, T, H);
+  p = SlidingArgs{};
+  p.q = q; p.k = k; p.v = v; p.lengths = lengths;
+  p.qb = strides[0]; p.qt = strides[1]; p.qh = strides[2];
+  p.kb = strides[3]; p.kt = strides[4]; p.kh = strides[5];
+  p.vb = strides[6]; p.vt = strides[7]; p.vh = strides[8];
+  p.B = B; p.T = T; p.H = H; p.G = G; p.D = D;
+  p.W = std::min(window, T);  // a window of T keys holds every earlier one
+  p.S = std::min(sinks, T);
+  p.scale = scale;
+  p.scale2 = scale * kLog2e;
+  return HATTN_OK;
+}
+
+size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+size_t sliding_bwd_delta(int B, int T, int H) { return up16((size_t)B * H * T * sizeof(float)); }
+
+// Workgroups that one row and key head's slots are cut into: enough that the card has
+// 1024 of them, where each keeps at least 128 slots (a tile for each of its waves).
+int step_splits(int B, int H, int G, int slots) {
+  const long base = (long)B * G * ((H / G + 15) / 16);
+  const long want = (1024 + base - 1) / base, most = (slots + 127) / 128;
+  return (int)std::max(1L, std::min(want, most));
+}
+
+}  // namespace
+
+extern "C" {
+
+int hattn_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                         void* y, void* s, float* mean, float* rstd, long long rows, int n,
+                         float eps, int dtype_x, int dtype_r, int dtype_w, void* stream) {
+  if (int st = norm_checks(rows, n, dtype_x, dtype_r, dtype_w, residual != nullptr)) return st;
+  if (!x || !y || (residual && !s) || !mean != !rstd) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  return check_hip(hattn_layer_norm_fwd_launch(x, residual, weight, bias, y, s, mean, rstd,
+                                               (long)rows, n, eps, dtype_x, dtype_r, dtype_w,
+                                               (hipStream_t)stream),
+                   "hattn_layer_norm_fwd launch");
+}
+
+size_t hattn_layer_norm_bwd_workspace(long long rows, int n) {
+  if (rows <= 0 || n <= 0 || n > kLayerNormMaxN) return 0;
+  return hattn_layer_norm_bwd_ws_bytes((long)rows, n);
+}
+
+int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, const float* rstd,
+                         const void* dy, const void* ds, void* dx, void* dresidual, void* dweight,
+                         void* dbias, long long rows, int n, int dtype_x, int dtype_s, int dtype_w,
+                         void* ws, size_t ws_bytes, void* stream) {
+  if (int st = norm_checks(rows, n, dtype_x, dtype_s, dtype_w, true)) return st;
+  if (!s || !mean || !rstd || !dy) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (dweight || dbias) {
+    const size_t need = hattn_layer_norm_bwd_ws_bytes((long)rows, n);
+    if (!ws || ws_bytes < need)
+      return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  }
+  return check_hip(hattn_layer_norm_bwd_launch(s, weight, mean, rstd, dy, ds, dx, dresidual, dweight,
+                                               dbias, (float*)ws, (long)rows, n, dtype_x, dtype_s,
+                                               dtype_w, (hipStream_t)stream),
+                   "hattn_layer_norm_bwd launch");
+}
+
+int hattn_gated_recurrence_segments(int T) { return T > 0 ? hattn_recurrence_segments(T) : 0; }
+
+size_t hattn_gated_recurrence_workspace(int B, int T, int D) {
+  if (recurrence_checks(B, T, D, HATTN_FP32, HATTN_FP32) != HATTN_OK) return 0;
+  return recurrence_ws(B, T, D);
+}
+
+int hattn_gated_recurrence_fwd(const void* x, const void* g, const float* h0, const int* lengths,
+                               void* o, float* ht, float* carry, int B, int T, int D, int dtype_x,
+                               int dtype_g, void* ws, size_t ws_bytes, void* stream) {
+  if (int st = recurrence_checks(B, T, D, dtype_x, dtype_g)) return st;
+  if (!x || !g || !o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  const size_t need = recurrence_ws(B, T, D);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned({ws}, 8)))
+    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  RecurrenceArgs p{};
+  p.x = x; p.g = g; p.h0 = h0; p.lengths = lengths; p.o = o; p.ht = ht; p.carry = carry; p.ws = ws;
+  p.B = B; p.T = T; p.D = D; p.strips = (D + 63) / 64; p.nseg = hattn_recurrence_segments(T);
+  return check_hip(hattn_recurrence_launch(0, p, dtype_x, dtype_g, (hipStream_t)stream),
+                   "hattn_gated_recurrence_fwd launch");
+}
+
+int hattn_gated_recurrence_bwd(const void* x, const void* g, const float* carry,
+                               const int* lengths, const void* dout, const float* dht, void* dx,
+                               void* dg, float* dh0, int B, int T, int D, int dtype_x, int dtype_g,
+                               void* ws, size_t ws_bytes, void* stream) {
+  if (int st = recurrence_checks(B, T, D, dtype_x, dtype_g)) return st;
+  if (!x || !g || !carry || !dout || !dx || !dg) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  const size_t need = recurrence_ws(B, T, D);
+  if (need > 0 && (!ws || ws_bytes < need || !aligned({ws}, 8)))
+    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  RecurrenceArgs p{};
+  p.x = x; p.g = g; p.go = dout; p.ght = dht; p.lengths = lengths; p.dx = dx; p.dg = dg;
+  p.dh0 = dh0; p.carry = const_cast<float*>(carry); p.ws = ws;
+  p.B = B; p.T = T; p.D = D; p.strips = (D + 63) / 64; p.nseg = hattn_recurrence_segments(T);
+  return check_hip(hattn_recurrence_launch(1, p, dtype_x, dtype_g, (hipStream_t)stream),
+                   "hattn_gated_recurrence_bwd launch");
+}
+
+int hattn_gated_recurrence_step(float* state, const void* x, const void* g, void* o, int B, int D,
+                                int dtype_x, int dtype_g, void* stream) {
+  if (int st = recurrence_checks(B, 1, D, dtype_x, dtype_g)) return st;
+  if (!state || !x || !g || !o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  RecurrenceArgs p{};
+  p.x = x; p.g = g; p.o = o; p.ht = state;
+  p.B = B; p.T = 1; p.D = D;
+  return check_hip(hattn_recurrence_launch(2, p, dtype_x, dtype_g, (hipStream_t)stream),
+                   "hattn_gated_recurrence_step launch");
+}
+
+int hattn_sliding_fwd(const void* q, const void* k, const void* v, const int* lengths,
+                      const long long* strides, void* o, float* lse, int B, int T, int H, int G,
+                      int D, int window, int sinks, float scale, int dtype, void* stream) {
+  SlidingArgs p;
+  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype))
+    return st;
+  if (!o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (!aligned({q, k, v, o}, 16)) return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
+  p.out = o;
+  p.lse = lse;
+  return check_hip(hattn_sliding_fwd_launch(p, dtype, (hipStream_t)stream),
+                   "hattn_sliding_fwd launch");
+}
+
+size_t hattn_sliding_bwd_workspace(int B, int T, int H, int G, int D, int window, int sinks) {
+  if (B <= 0 || T <= 0 || D <= 0 || window < 1 || sinks < 0 || G <= 0 || H < G) return 0;
+  const int S = std::min(sinks, T);
+  return sliding_bwd_delta(B, T, H) + (size_t)sliding_sink_slots(T, H, G, std::min(window, T), S) *
+                                          B * G * S * 2 * D * sizeof(float);
+}
+
+int hattn_sliding_bwd(const void* q, const void* k, const void* v, const int* lengths,
+                      const long long* strides, const void* o, const float* lse, const void* dout,
+                      void* dq, void* dk, void* dv, int B, int T, int H, int G, int D, int window,
+                      int sinks, float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  SlidingArgs p;
+  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype))
+    return st;
+  if (!o || !lse || !dout || !dq || !dk || !dv) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (!aligned({q, k, v, o, dout, dq, dk, dv, ws}, 16))
+    return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
+  const size_t need = hattn_sliding_bwd_workspace(B, T, H, G, D, window, sinks);
+  if (!ws || ws_bytes < need)
+    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  p.o = o; p.go = dout; p.lse = const_cast<float*>(lse);
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.delta = (float*)ws;
+  if (sliding_sink_slots(T, H, G, p.W, p.S) > 0)
+    p.part = (float*)((char*)ws + sliding_bwd_delta(B, T, H));
+  return check_hip(hattn_sliding_bwd_launch(p, dtype, (hipStream_t)stream),
+                   "hattn_sliding_bwd launch");
+}
+
+int hattn_sliding_cache_fill(const void* k, const void* v, const int* lengths,
+                             const long long* strides, void* k_cache, void* v_cache, int* counts,
+                             int B, int T, int G, int D, int window, int sinks, int dtype,
+                             void* stream) {
+  if (T <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
+  if (int st = sliding_checks(B, G, G, D, window, sinks, 1.f, dtype)) return st;
+  if (!k || !v || !strides || !k_cache || !v_cache || !counts)
+    return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (int st = stride_checks(strides, 6)) return st;
+  if (!aligned({k, v, k_cache, v_cache}, 16))
+    return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
+  if ((long long)window + sinks > INT_MAX ||
+      (long long)B * G * ((long long)sinks + window) * (D / 8) / 256 >= INT_MAX)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d G=%d window=%d: cache too large", B, G, window);
+  SlidingStepArgs p{};
+  p.k = k; p.v = v; p.kc = k_cache; p.vc = v_cache; p.counts = counts;
+  p.B = B; p.G = G; p.D = D; p.W = window; p.S = sinks;
+  long st[6];
+  for (int i = 0; i < 6; ++i) st[i] = (long)strides[i];
+  return check_hip(hattn_sliding_cache_launch(p, T, st, lengths, (hipStream_t)stream),
+                   "hattn_sliding_cache_fill launch");
+}
+
+size_t hattn_sliding_step_workspace(int B, int H, int G, int D, int window, int sinks) {
+  if (B <= 0 || G <= 0 || H < G || D <= 0 || window < 1 || sinks < 0 ||
+      (long long)window + sinks > INT_MAX)
+    return 0;
+  return (size_t)B * H * step_splits(B, H, G, window + sinks) * (D + 2) * sizeof(float);
+}
+
+int hattn_sliding_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                       int* counts, void* o, int B, int H, int G, int D, int window, int sinks,
+                       float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  if (int st = sliding_checks(B, H, G, D, window, sinks, scale, dtype)) return st;
+  if (!q || !k || !v || !k_cache || !v_cache || !counts || !o)
+    return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (!aligned({q, k, v, k_cache, v_cache, ws}, 16))
+    return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
+  if ((long long)window + sinks > INT_MAX - 256)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "window=%d too large", window);
+  const size_t need = hattn_sliding_step_workspace(B, H, G, D, window, sinks);
+  if (!ws || ws_bytes < need)
+    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  SlidingStepArgs p{};
+  p.q = q; p.k = k; p.v = v; p.kc = k_cache; p.vc = v_cache; p.counts = counts; p.o = o;
+  p.B = B; p.H = H; p.G = G; p.D = D; p.W = window; p.S = sinks;
+  p.splits = step_splits(B, H, G, window + sinks);
+  p.rblocks = (H / G + 15) / 16;
+  if ((long long)B * G * p.rblocks * p.splits > INT_MAX || (long long)B * H > INT_MAX)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d H=%d: too many rows", B, H);
+  p.scale2 = scale * kLog2e;
+  p.part = (float*)ws;
+  p.stat = p.part + (size_t)B * H * p.splits * D;
+  return check_hip(hattn_sliding_step_launch(p, dtype, (hipStream_t)stream),
+                   "hattn_sliding_step launch");
+}
+
+}  // extern "C"

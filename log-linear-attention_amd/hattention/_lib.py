@@ -81,6 +81,20 @@ SIGNATURES = [
     ("hattn_gated_rmsnorm_bwd_workspace", _S, [_LL, _I]),
     ("hattn_gated_rmsnorm_bwd", _I, [_P, _P, _LL, _P, _P, _P, _P, _P, _LL, _P, _LL, _I] + [_I] * 6
      + [_P, _S, _P]),
+    ("hattn_layer_norm_fwd", _I, [_P] * 8 + [_LL, _I, ctypes.c_float] + [_I] * 3 + [_P]),
+    ("hattn_layer_norm_bwd_workspace", _S, [_LL, _I]),
+    ("hattn_layer_norm_bwd", _I, [_P] * 10 + [_LL, _I] + [_I] * 3 + [_P, _S, _P]),
+    ("hattn_gated_recurrence_segments", _I, [_I]),
+    ("hattn_gated_recurrence_workspace", _S, [_I] * 3),
+    ("hattn_gated_recurrence_fwd", _I, [_P] * 7 + [_I] * 5 + [_P, _S, _P]),
+    ("hattn_gated_recurrence_bwd", _I, [_P] * 9 + [_I] * 5 + [_P, _S, _P]),
+    ("hattn_gated_recurrence_step", _I, [_P] * 4 + [_I] * 4 + [_P]),
+    ("hattn_sliding_fwd", _I, [_P] * 7 + [_I] * 7 + [ctypes.c_float, _I, _P]),
+    ("hattn_sliding_bwd_workspace", _S, [_I] * 7),
+    ("hattn_sliding_bwd", _I, [_P] * 11 + [_I] * 7 + [ctypes.c_float, _I, _P, _S, _P]),
+    ("hattn_sliding_cache_fill", _I, [_P] * 7 + [_I] * 7 + [_P]),
+    ("hattn_sliding_step_workspace", _S, [_I] * 6),
+    ("hattn_sliding_step", _I, [_P] * 7 + [_I] * 6 + [ctypes.c_float, _I, _P, _S, _P]),
 ]
 
 _lock = threading.Lock()
@@ -159,6 +173,16 @@ def stream_handle(device: torch.device) -> int:
         return _raw_stream(device.index if device.index is not None
                            else torch.cuda.current_device())
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(dev: torch.device, fn, *args) -> None:
+    """Calls an entry point that ends in a stream argument on the current stream of
+    ``dev``, with ``dev`` as the current device."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        check(fn(*args, stream_handle(dev)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, stream_handle(dev)))
 
 
 def fwd_status(ws, B: int, T: int, H: int, V: int, device: torch.device) -> int:
