@@ -72,11 +72,17 @@ int sliding_checks(int B, int H, int G, int D, int window, int sinks, float scal
   return HATTN_OK;
 }
 
+const long long kMaxTokenStride = 1LL << 24;
+
 // Strides in elements, batch / token / head of q, k, v: 16-byte rows.
 int stride_checks(const long long* st, int n) {
   for (int i = 0; i < n; ++i)
-    if (st[i] % 8 != 0)
+    if (st[i] % 8 != 0 || st[i] < 0)
       return fail(HATTN_ERR_VALUE, "stride %lld is not a multiple of 8 elements", st[i]);
+  // the rows of one tile are addressed by 32-bit offsets
+  for (int i = 1; i < n; i += 3)
+    if (st[i] >= kMaxTokenStride)
+      return fail(HATTN_ERR_NOT_IMPLEMENTED, "token stride %lld of 2^24 elements or more", st[i]);
   return HATTN_OK;
 }
 

@@ -13,13 +13,16 @@
 //
 // A query that sees one key has P = 1 and dS = 0 whatever its scores: dP - delta is not
 // left to cancel there.
+#include <climits>
+
 #include "sliding_device.h"
 
 namespace hattn {
 
 template <typename E, int DP>
-__global__ __launch_bounds__(256, 2) void sliding_bwd_q_kernel(SlidingArgs p) {
-  __shared__ __attribute__((aligned(16))) __bf16 K0[64 * DP], V0[64 * DP], K1[64 * DP], V1[64 * DP];
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void sliding_bwd_q_kernel(SlidingArgs p) {
+  constexpr int BN = 32;
+  __shared__ __attribute__((aligned(16))) __bf16 K0[BN * DP], V0[BN * DP], K1[BN * DP], V1[BN * DP];
   const int lane = threadIdx.x & 63, ln = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = p.H / p.G, nblk = (p.T + 127) / 128;
@@ -59,27 +62,23 @@ __global__ __launch_bounds__(256, 2) void sliding_bwd_q_kernel(SlidingArgs p) {
   }
   const float lse = p.lse[stat + tc];
   const bool alone = t == 0 || (p.W == 1 && p.S == 0);
-  const KeyList keys(t0, len, p.W, p.S);
-  const int tiles = (keys.n + 63) / 64;
+  const KeyList<BN> keys(t0, 128, len, p.W, p.S);
+  const int tiles = keys.tiles();
 
+  const TileLoad<DP, BN, 4> tile(p.D);
   const auto stage = [&](int j, __bf16* K, __bf16* V) __attribute__((always_inline)) {
-    constexpr int RPI = 512 / DP, N = DP / 32;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = wave * N + i, rw = at * RPI + lane / (DP / 8);
-      const long pos = keys.pos(min(64 * j + rw, keys.n - 1));
-      load_rows<DP>(k + pos * p.kt, rw, p.D, K + at * 512);
-      load_rows<DP>(v + pos * p.vt, rw, p.D, V + at * 512);
-    }
+    keys.load(tile, j, k, p.kt, K);
+    keys.load(tile, j, v, p.vt, V);
   };
-  const auto step = [&](int j, const __bf16* K, const __bf16* V, __bf16* Kn, __bf16* Vn)
+  const auto step = [&](auto MASK, int j, const __bf16* K, const __bf16* V, __bf16* Kn, __bf16* Vn)
                         __attribute__((always_inline)) {
     tile_barrier();
     if (j + 1 < tiles) stage(j + 1, Kn, Vn);
-    const int kind = tile_kind(keys, j, tw, p.W, p.S);
+    int kind = kFull;
+    if constexpr (MASK.value) kind = tile_kind(keys, j, tw, p.W, p.S);
     if (kind == kSkip) return;
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < BN / 32; ++kt) {
       floatx16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) s = mfma32<E>(row_frag<DP>(K, 32 * kt, c), qf[c], s);
@@ -87,13 +86,12 @@ __global__ __launch_bounds__(256, 2) void sliding_bwd_q_kernel(SlidingArgs p) {
       for (int c = 0; c < DP / 16; ++c) dp = mfma32<E>(row_frag<DP>(V, 32 * kt, c), gf[c], dp);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = exp2_(s[i] * p.scale2 - lse) * (dp[i] - delta);
-      if (kind == kMask) {
+      if constexpr (MASK.value) {
+        if (kind == kMask) {
+          const TileMask seen(keys, j, t, p.W, p.S);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int slot = 64 * j + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
-          const int pos = keys.pos(slot);
-          const bool seen = slot < keys.n && pos <= t && (pos + p.W > t || pos < p.S) && !alone;
-          s[i] = seen ? s[i] : 0.f;
+          for (int i = 0; i < 16; ++i)
+            s[i] = seen(32 * kt + 8 * (i >> 2) + (i & 3)) & !alone ? s[i] : 0.f;
         }
       }
 #pragma unroll
@@ -106,10 +104,16 @@ __global__ __launch_bounds__(256, 2) void sliding_bwd_q_kernel(SlidingArgs p) {
     }
   };
   stage(0, K0, V0);
-  for (int j = 0; j < tiles; j += 2) {
-    step(j, K0, V0, K1, V1);
-    if (j + 1 < tiles) step(j + 1, K1, V1, K0, V0);
-  }
+  int j = 0;
+  const auto pairs = [&](auto MASK) __attribute__((always_inline)) {
+    step(MASK, j, K0, V0, K1, V1);
+    if (j + 1 < tiles) step(MASK, j + 1, K1, V1, K0, V0);
+  };
+  // where each query sees one key, every tile is masked
+  const int lo = keys.first_whole(t0, 128, p.W), hi = alone ? 0 : keys.end_whole(t0);
+  for (; j < tiles && !(j >= lo && j + 2 <= hi); j += 2) pairs(Bool<true>());
+  for (; j + 2 <= hi; j += 2) pairs(Bool<false>());
+  for (; j < tiles; j += 2) pairs(Bool<true>());
   if (t < p.T) store_t<E, DP>(dq, acc, t < len ? p.scale : 0.f, p.D);
 }
 
@@ -154,25 +158,22 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
   floatx16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = dv[dt] = zero16();
+  const bool alone = p.W == 1 && p.S == 0;  // every query sees one key
   const int per = end > first ? (end - first + QT - 1) / QT : 0;  // tiles of one head
   const int tiles = per * heads;
 
+  const TileLoad<DP, QT, 4> tile(p.D);
   const auto stage = [&](int j, __bf16* Q, __bf16* O, float* st) __attribute__((always_inline)) {
-    constexpr int RPI = 512 / DP, N = QT / RPI / 4;
     const int h = h0 + j / per, tq = first + j % per * QT;
     const __bf16* q = (const __bf16*)p.q + b * p.qb + h * p.qh;
     const __bf16* go = (const __bf16*)p.go + ((long)b * p.T * p.H + h) * p.D;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = wave * N + i, rw = at * RPI + lane / (DP / 8);
-      const long t = min(tq + rw, end - 1);
-      load_rows<DP>(q + t * p.qt, rw, p.D, Q + at * 512);
-      load_rows<DP>(go + t * p.H * p.D, rw, p.D, O + at * 512);
-    }
-    // lse and delta of 64 rows a wave and load
+    tile.run(q, p.qt, tq, end - 1, Q);
+    tile.run(go, (long)p.H * p.D, tq, end - 1, O);
+    // lse and delta of the tile's rows, 64 values a wave
     if (wave < 2 * QT / 64) {
-      const float* src = (wave < QT / 64 ? p.lse : p.delta) + ((long)b * p.H + h) * p.T;
-      const int t = min(tq + wave % (QT / 64) * 64 + lane, end - 1);
+      const int i = 64 * wave + lane;
+      const float* src = (i < QT ? p.lse : p.delta) + ((long)b * p.H + h) * p.T;
+      const int t = min(tq + i % QT, end - 1);
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + t),
                                        (__attribute__((address_space(3))) void*)(st + 64 * wave), 4,
                                        0, 0);
@@ -185,11 +186,11 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
     const int tq = first + j % per * QT;
 #pragma unroll
     for (int u = 0; u < (SINKS ? 1 : 2); ++u) {
+      // the queries tw .. tw + 31 against the wave's keys
       const int q0 = SINKS ? 32 * wave : 32 * u, tw = tq + q0;
-      // the wave's keys kw .. kw + 31 against the queries tw .. tw + 31
       if (tw >= end || (!SINKS && (tw + 31 < kw || tw >= kw + 31 + p.W))) continue;
-      const bool mask = SINKS ? tw + 31 >= end || tw - kw - 31 < p.W
-                              : tw < kw + 31 || tw + 31 >= kw + p.W || tw + 31 >= end;
+      const bool mask = alone || tw == 0 || tw + 31 >= end ||
+                        (SINKS ? tw - kw - 31 < p.W : tw < kw + 31 || tw + 31 >= kw + p.W);
       floatx16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) s = mfma32<E>(row_frag<DP>(Q, q0, c), kf[c], s);
@@ -206,13 +207,15 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
         }
       }
       if (mask) {
-        const bool one = p.W == 1 && p.S == 0;
+        // query tw + 4 hf + place sees the key from place >= low on, up to place <= up
+        const int from = tw + 4 * hf, up = SINKS ? end - 1 - from : min(end, key + p.W) - 1 - from;
+        const int low = SINKS ? key + p.W - from : key - from, one = alone ? INT_MAX : -from;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int t = tw + 8 * (i >> 2) + 4 * hf + (i & 3);
-          const bool seen = t < end && (SINKS ? t - key >= p.W : key <= t && t - key < p.W);
+          const int place = 8 * (i >> 2) + (i & 3);
+          const bool seen = (place >= low) & (place <= up);
           s[i] = seen ? s[i] : 0.f;
-          dp[i] = seen && t > 0 && !one ? dp[i] : 0.f;
+          dp[i] = seen & (place > one) ? dp[i] : 0.f;
         }
       }
 #pragma unroll

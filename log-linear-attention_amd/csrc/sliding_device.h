@@ -43,6 +43,14 @@ __device__ __forceinline__ floatx16 zero16() {
   return z;
 }
 
+// max(a, b, c) as one instruction: fmaxf would first quiet each operand by one of its own.
+// A NaN operand is ignored.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Eight values (registers 8 s .. 8 s + 7 of a D tile) as a 16-bit operand.
@@ -80,22 +88,61 @@ __device__ __forceinline__ bf16x8 tr32(const __bf16* X, int r0, int d0) {
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// Starts the asynchronous load of 512 / DP rows into 1 KB of LDS at dst (the same in
-// every lane): lane i fills 16 bytes at dst + 16 i.  src: this lane's row; row: its
-// index in the tile.  Pieces past D read the row's first: the other operand is zero
-// there, or the result is not stored.
-template <int DP>
-__device__ __forceinline__ void load_rows(const __bf16* src, int row, int D, __bf16* dst) {
-  const int c = ((threadIdx.x & 63) % (DP / 8)) ^ swizzle<DP>(row);
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void*)(src + (c * 8 < D ? c * 8 : 0)),
-      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+// Asynchronous loads of a tile of ROWS rows by the workgroup's NW waves.  A load fills
+// 1 KB of LDS, lane i the 16 bytes at 16 i: 512 / DP rows.  Pieces past D read the row's
+// first: the other operand is zero there, or the result is not stored.
+template <int DP, int ROWS, int NW>
+struct TileLoad {
+  static constexpr int RPI = 512 / DP, N = ROWS / RPI / NW;  // rows a load, loads a wave
+  int wave;
+  unsigned piece[N];  // bytes into its row that this lane reads
+  __device__ __forceinline__ explicit TileLoad(int D)
+      : wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (threadIdx.x & 63) % (DP / 8) ^ swizzle<DP>(row(i));
+      piece[i] = c * 8 < D ? c * 16 : 0;
+    }
+  }
+  __device__ __forceinline__ int row(int i) const {
+    return (wave * N + i) * RPI + (threadIdx.x & 63) / (DP / 8);
+  }
+  // src: the row of this lane's load i, as bytes from a base that all lanes share
+  __device__ __forceinline__ void load(const char* base, unsigned src, int i, __bf16* X) const {
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(base + (src + piece[i])),
+        (__attribute__((address_space(3))) void*)(X + (wave * N + i) * 512), 16, 0, 0);
+  }
+  // rows first .. first + ROWS - 1 of a matrix with a token stride of `stride` elements; those
+  // past `last` read it
+  __device__ __forceinline__ void run(const __bf16* base, long stride, int first, int last,
+                                      __bf16* X) const {
+    const char* at = (const char*)(base + first * stride);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      load(at, (unsigned)min(row(i), last - first) * (unsigned)(2 * stride), i, X);
+  }
+};
+
+// Waits until at most N of this wave's loads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 16);
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
 }
 
 // Waits for this wave's asynchronous loads, then for the other waves.
 __device__ __forceinline__ void tile_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  wait_loads<0>();
   __syncthreads();
+}
+
+// A barrier that leaves asynchronous loads in flight (__syncthreads waits for them): this
+// wave's reads of LDS are done before it, and none moves across it.
+__device__ __forceinline__ void phase_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // The B operand rows of one matrix, kept in registers: row `src` of this lane (ln),
@@ -141,27 +188,72 @@ __device__ __forceinline__ int row_length(const SlidingArgs& p, int b) {
   return p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
 }
 
-// The keys of the 128 queries from t0 on, as one list without holes: the sinks that lie
-// before the window, then the window [lo, hi).
+// The keys of `block` queries from t0 on, as one list without holes: the sinks that lie
+// before the window, then the window [lo, hi); tiles of BN keys.
+template <int BN>
 struct KeyList {
   int ns, lo, n;
-  __device__ __forceinline__ KeyList(int t0, int len, int W, int S) {
+  __device__ __forceinline__ KeyList(int t0, int block, int len, int W, int S) {
     lo = max(0, t0 - W + 1);
     ns = min(S, lo);
-    n = ns + min(len, t0 + 128) - lo;
+    n = ns + min(len, t0 + block) - lo;
   }
   __device__ __forceinline__ int pos(int slot) const {
     return slot < ns ? slot : slot - ns + lo;
   }
+  // The tiles that all of the block's queries see whole, from the first to before the end
+  // (none where the end is not above the first).
+  __device__ __forceinline__ int first_whole(int t0, int block, int W) const {
+    return (ns + max(0, t0 + block - W - lo) + BN - 1) / BN;
+  }
+  __device__ __forceinline__ int end_whole(int t0) const { return (ns + t0 + 1 - lo) / BN; }
+  __device__ __forceinline__ int tiles() const { return (n + BN - 1) / BN; }
+  // Starts the loads of keys BN j .. BN j + BN - 1 of the list.  Tiles with sinks may have a
+  // hole between them and the window.
+  template <typename Tile>
+  __device__ __forceinline__ void load(const Tile& tile, int j, const __bf16* x, long stride,
+                                       __bf16* X) const {
+    if (BN * j < ns) {
+#pragma unroll
+      for (int i = 0; i < tile.N; ++i)
+        tile.load((const char*)(x + pos(min(BN * j + tile.row(i), n - 1)) * stride), 0, i, X);
+    } else {
+      tile.run(x, stride, BN * j - ns + lo, n - 1 - ns + lo, X);
+    }
+  }
 };
 
-// What a wave's 32 queries from tw on need of keys [64 j, 64 j + 64) of the list.
+// What a wave's 32 queries from tw on need of tile j of the list.
 enum { kSkip, kFull, kMask };
-__device__ __forceinline__ int tile_kind(const KeyList& keys, int j, int tw, int W, int S) {
-  const int s0 = 64 * j, s1 = min(s0 + 63, keys.n - 1);
+template <int BN>
+__device__ __forceinline__ int tile_kind(const KeyList<BN>& keys, int j, int tw, int W, int S) {
+  const int s0 = BN * j, s1 = min(s0 + BN - 1, keys.n - 1);
   const int first = keys.pos(s0), last = keys.pos(s1), near = keys.pos(max(s0, keys.ns));
   if (first > tw + 31 || (first >= S && last + W <= tw)) return kSkip;
-  return s1 < s0 + 63 || last > tw || near + W <= tw + 31 ? kMask : kFull;
+  return s1 < s0 + BN - 1 || last > tw || near + W <= tw + 31 ? kMask : kFull;
 }
+
+// Which keys of a masked tile this lane's query t sees, by the key's place 8 (i >> 2) + (i & 3)
+// + 32 kt after BN j + 4 hf: from the window's first (low < place) or as a sink (place < sink),
+// up to its own (place <= up).  Sinks are the list's first S slots, whether they lie before
+// the window or in it, and the hole after them lies before every query.
+struct TileMask {
+  int up, low, sink;
+  template <int BN>
+  __device__ __forceinline__ TileMask(const KeyList<BN>& keys, int j, int t, int W, int S) {
+    const int from = BN * j + 4 * (threadIdx.x >> 5 & 1), at = from + keys.lo - keys.ns;
+    up = min(t - at, keys.n - 1 - from);
+    low = t - W - at;
+    sink = S - from;
+  }
+  __device__ __forceinline__ bool operator()(int place) const {
+    return (place <= up) & ((place > low) | (place < sink));
+  }
+};
+
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
 
 }  // namespace hattn

@@ -21,7 +21,8 @@ MAX_SINKS = 64
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t where its rows start on 16 bytes and are contiguous, else a copy that does."""
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1):
+            all(s % 8 == 0 for n, s in zip(t.shape[:-1], t.stride()) if n > 1) and \
+            t.stride(1) < 2 ** 24:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()

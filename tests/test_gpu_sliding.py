@@ -170,7 +170,18 @@ def test_views_are_read_in_place():
     k1 = k[:, :, :1].detach().requires_grad_()
     o = sliding_window_attention(q, k1.expand(B, T, H, D), v[:, :, :1].expand(B, T, H, D), 40, 4)
     o2 = sliding_window_attention(q, k1, v[:, :, :1], 40, 4)
-    assert torch.equal(o, o2)
+    # the head layouts may take different tiles, so they agree to the bound and not to the bit
+    want, tol = oracle(q, k1.detach(), v[:, :, :1], 40, 4, None, None, do)
+    close("o", o.detach(), want["o"], tol["o"])
+    close("o2", o2.detach(), want["o"], tol["o"])
+    (dk,) = torch.autograd.grad(o2, [k1], do)
+    close("dk", dk, want["dk"], tol["dk"])
+    (dk,) = torch.autograd.grad(o, [k1], do)
+    # H gradients of their own, each rounded, added in bf16 (H - 1 more roundings)
+    mine, each = oracle(q, k1.detach().expand(B, T, H, D), v[:, :, :1].expand(B, T, H, D), 40, 4,
+                        None, None, do)
+    mag = mine["dk"].abs().sum(2, keepdim=True)
+    close("dk", dk, want["dk"], each["dk"].sum(2, keepdim=True) + H * 2.0 ** -8 * mag)
 
 
 def test_padding_is_not_read():
