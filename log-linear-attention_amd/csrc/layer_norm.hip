@@ -8,6 +8,8 @@
 
 namespace hattn {
 
+constexpr long kNormFwdGrid = 2048;  // eight workgroups a CU; more only read the parameters again
+
 template <typename TX, typename TR, bool RES, int VEC, int NW, int CH>
 __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
     const TX* __restrict__ x, const TR* __restrict__ res, const void* __restrict__ weight,
@@ -21,13 +23,10 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
   constexpr int STEP = 64 * NW * VEC;
   float w[CH][VEC], b[CH][VEC];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int at = first + c * STEP + i;
-      w[c][i] = weight && at < n ? load_param(weight, dtype_w, at) : 1.f;
-      b[c][i] = bias && at < n ? load_param(bias, dtype_w, at) : 0.f;
-    }
+  for (int c = 0; c < CH; ++c) {
+    load_params<VEC>(weight, dtype_w, first + c * STEP, n, 1.f, w[c]);
+    load_params<VEC>(bias, dtype_w, first + c * STEP, n, 0.f, b[c]);
+  }
   const float inv_n = 1.f / (float)n;
   for (long row = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); row < rows;
        row += (long)gridDim.x * RPB) {
@@ -87,7 +86,7 @@ static hipError_t launch_fwd(const void* x, const void* res, const void* weight,
   const NormShape sh = norm_shape(rows, n, n % 8 == 0 && bits % 16 == 0);
   const long rpb = 4 / sh.nw;
   const long want = (rows + rpb - 1) / rpb;
-  const dim3 grid((unsigned)(want < 4096 ? want : 4096));
+  const dim3 grid((unsigned)(want < kNormFwdGrid ? want : kNormFwdGrid));
 #define CALL(VEC, NW, CH)                                                                      \
   hipLaunchKernelGGL((layer_norm_fwd_kernel<TX, TR, RES, VEC, NW, CH>), grid, dim3(256), 0,    \
                      stream, (const TX*)x, (const TR*)res, weight, bias, (TX*)y, (TR*)s, mean, \

@@ -10,8 +10,6 @@
 
 namespace hattn {
 
-constexpr int kNormBwdGrid = 512;  // workgroups, and so partial rows, at most
-
 template <typename TX, typename TS, bool DS, int VEC, int NW, int CH>
 __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
     const TS* __restrict__ s, const void* __restrict__ weight, const float* __restrict__ mean_in,
@@ -26,13 +24,11 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
   constexpr int STEP = 64 * NW * VEC;
   float w[CH][VEC], dw[CH][VEC], db[CH][VEC];
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
+  for (int c = 0; c < CH; ++c) {
+    load_params<VEC>(weight, dtype_w, first + c * STEP, n, 1.f, w[c]);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int at = first + c * STEP + i;
-      w[c][i] = weight && at < n ? load_param(weight, dtype_w, at) : 1.f;
-      dw[c][i] = db[c][i] = 0.f;
-    }
+    for (int i = 0; i < VEC; ++i) dw[c][i] = db[c][i] = 0.f;
+  }
   const float inv_n = 1.f / (float)n;
   int turn = 0;
   for (long row = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); row < rows;
@@ -119,8 +115,16 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_join_kernel(const float* _
   __shared__ float sm[16][17];
   const int col = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
   float a = 0.f;
-  if (col < 2 * n)
-    for (int p = r; p < nparts; p += 16) a += part[(long)p * 2 * n + col];
+  if (col < 2 * n) {
+    // eight loads in flight: the sum is short and waits for memory
+    float x[8];
+    for (int p = r; p < nparts; p += 128) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p + 16 * i < nparts ? part[(long)(p + 16 * i) * 2 * n + col] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a += x[i];
+    }
+  }
   sm[r][threadIdx.x & 15] = a;
   __syncthreads();
   if (r == 0 && col < 2 * n) {
@@ -136,7 +140,8 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_join_kernel(const float* _
 
 static long norm_bwd_grid(long rows, const NormShape& sh) {
   const long want = (rows + 4 / sh.nw - 1) / (4 / sh.nw);
-  return want < kNormBwdGrid ? want : kNormBwdGrid;
+  const long most = sh.nw == 1 ? kNormBwdGrid1 : kNormBwdGrid4;
+  return want < most ? want : most;
 }
 
 template <typename TX, typename TS, bool DS>
@@ -166,9 +171,9 @@ static hipError_t launch_bwd(const void* s, const void* weight, const float* mea
 }  // namespace hattn
 
 size_t hattn_layer_norm_bwd_ws_bytes(long rows, int n) {
-  // the largest grid of any shape: four rows a workgroup or one
-  const long parts = rows < hattn::kNormBwdGrid ? rows : hattn::kNormBwdGrid;
-  return (size_t)parts * 2 * n * sizeof(float);
+  // the larger grid of the two that the tensors' alignment leaves open
+  const long most = rows > 1024 && n <= 2048 ? hattn::kNormBwdGrid1 : hattn::kNormBwdGrid4;
+  return (size_t)(rows < most ? rows : most) * 2 * n * sizeof(float);
 }
 
 hipError_t hattn_layer_norm_bwd_launch(const void* s, const void* weight, const float* mean,

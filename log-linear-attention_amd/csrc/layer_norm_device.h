@@ -56,6 +56,25 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[VEC]) {
   }
 }
 
+// VEC elements of a parameter from element `at` on, x in each where there is none.
+template <int VEC>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int at, int n, float x,
+                                            float (&out)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = x;
+  if (!p || at >= n) return;
+  if constexpr (VEC == 8) {
+    if ((uintptr_t)p % 16 == 0) {  // n is a multiple of 8, so the eight are there
+      if (dtype == 0) load_row<__bf16, 8>((const __bf16*)p + at, out);
+      else if (dtype == 1) load_row<_Float16, 8>((const _Float16*)p + at, out);
+      else load_row<float, 8>((const float*)p + at, out);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = load_param(p, dtype, at + i);
+}
+
 // Sum over the 64 lanes, in every lane.
 __device__ __forceinline__ float wave_sum(float x) { return sum_lq(row_sum16(x)); }
 
@@ -82,6 +101,10 @@ __device__ __forceinline__ void row_sums(float (&x)[NV], float* red) {
   }
 }
 
+// Workgroups of the backward at most, each of which writes one partial row of the parameters'
+// gradients: 1024 where a wave has its own rows, 512 where four waves share one.
+constexpr int kNormBwdGrid1 = 1024, kNormBwdGrid4 = 512;
+
 // How a row of n elements is spread over lanes: VEC elements a lane and load
 // (8, or 1 where rows do not start on 16 bytes), NW waves of the workgroup's
 // four on one row, CH loads a lane.  One wave a row up to 2048 elements; four
@@ -93,7 +116,7 @@ inline NormShape norm_shape(long rows, int n, bool vec) {
   if (!vec) return {1, 4, n <= 1024 ? 4 : n <= 4096 ? 16 : 64};
   const int nw = n > 2048 || rows <= 1024 ? 4 : 1;
   const int need = (n + 512 * nw - 1) / (512 * nw);
-  return {8, nw, need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8};
+  return {8, nw, need <= 4 ? need : need <= 6 ? 6 : 8};
 }
 
 }  // namespace hattn
@@ -108,11 +131,14 @@ inline NormShape norm_shape(long rows, int n, bool vec) {
     } else if ((sh).nw == 1) {                                     \
       if ((sh).ch == 1) { CALL(8, 1, 1); }                         \
       else if ((sh).ch == 2) { CALL(8, 1, 2); }                    \
+      else if ((sh).ch == 3) { CALL(8, 1, 3); }                    \
       else { CALL(8, 1, 4); }                                      \
     } else {                                                       \
       if ((sh).ch == 1) { CALL(8, 4, 1); }                         \
       else if ((sh).ch == 2) { CALL(8, 4, 2); }                    \
+      else if ((sh).ch == 3) { CALL(8, 4, 3); }                    \
       else if ((sh).ch == 4) { CALL(8, 4, 4); }                    \
+      else if ((sh).ch == 6) { CALL(8, 4, 6); }                    \
       else { CALL(8, 4, 8); }                                      \
     }                                                              \
   } while (0)

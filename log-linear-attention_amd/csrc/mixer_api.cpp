@@ -117,7 +117,7 @@ size_t sliding_bwd_delta(int B, int T, int H) { return up16((size_t)B * H * T * 
 int step_splits(int B, int H, int G, int slots) {
   const long base = (long)B * G * ((H / G + 15) / 16);
   const long want = (1024 + base - 1) / base, most = (slots + 127) / 128;
-  return (int)std::max(1L, std::min(want, most));
+  return (int)std::max(1L, std::min({want, most, (long)kStepSplits}));
 }
 
 }  // namespace

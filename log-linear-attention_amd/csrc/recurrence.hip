@@ -120,7 +120,7 @@ __device__ __forceinline__ Place place(const RecurrenceArgs& p, bool backward) {
 }
 
 template <typename TX, typename TG>
-__global__ __launch_bounds__(512, 4) void recurrence_fwd_kernel(RecurrenceArgs p) {
+__global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(RecurrenceArgs p) {
   __shared__ Map maps[kWaves][64];
   __shared__ float enter[64];
   const Place at = place(p, false);
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(512, 4) void recurrence_fwd_kernel(RecurrenceArgs p
 }
 
 template <typename TX, typename TG>
-__global__ __launch_bounds__(512) void recurrence_bwd_kernel(RecurrenceArgs p) {
+__global__ __launch_bounds__(64 * kWaves) void recurrence_bwd_kernel(RecurrenceArgs p) {
   __shared__ Map fwd[kWaves][64], bwd[kWaves][64];
   __shared__ float enter[64];
   const Place at = place(p, true);
@@ -294,9 +294,9 @@ static hipError_t launch(int what, const RecurrenceArgs& p, hipStream_t stream) 
   }
   const dim3 grid((unsigned)(units * p.nseg));
   if (what == 0)
-    hipLaunchKernelGGL((recurrence_fwd_kernel<TX, TG>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((recurrence_fwd_kernel<TX, TG>), grid, dim3(64 * kWaves), 0, stream, p);
   else
-    hipLaunchKernelGGL((recurrence_bwd_kernel<TX, TG>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL((recurrence_bwd_kernel<TX, TG>), grid, dim3(64 * kWaves), 0, stream, p);
   return hipGetLastError();
 }
 

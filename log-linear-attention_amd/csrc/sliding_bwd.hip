@@ -289,8 +289,13 @@ template <typename E>
 __global__ __launch_bounds__(256) void sliding_bwd_sinks_kernel(SlidingArgs p, int slots) {
   const long n = (long)p.B * p.G * p.S * 2 * p.D, i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
-  float x = 0.f;
-  for (int s = 0; s < slots; ++s) x += p.part[s * n + i];
+  float x = 0.f, y[8];
+  for (int s = 0; s < slots; s += 8) {  // eight loads in flight: the sum waits for memory
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y[u] = s + u < slots ? p.part[(s + u) * n + i] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x += y[u];
+  }
   const int d = i % p.D, which = i / p.D % 2, key = i / (2 * p.D) % p.S;
   const long bg = i / (2 * p.D) / p.S, b = bg / p.G, g = bg % p.G;
   const long at = ((b * p.T + key) * p.G + g) * p.D + d;

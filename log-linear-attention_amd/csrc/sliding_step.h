@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime.h>
 
+constexpr int kStepSplits = 256;  // workgroups that one row and key head's slots are cut into, at most
+
 struct SlidingStepArgs {
   const void *q, *k, *v;  // step: q [B, H, D], k, v [B, G, D]
   void *kc, *vc;          // [B, G, S + W, D]

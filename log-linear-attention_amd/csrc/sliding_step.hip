@@ -189,21 +189,37 @@ __global__ __launch_bounds__(256, 2) void sliding_step_kernel(SlidingStepArgs p)
   }
 }
 
-// Joins a head's partial results and advances its row's count.
+// Joins a head's partial results and advances its row's count; one thread an element.
 template <typename E>
-__global__ __launch_bounds__(64) void sliding_step_join_kernel(SlidingStepArgs p) {
+__global__ __launch_bounds__(128) void sliding_step_join_kernel(SlidingStepArgs p) {
+  __shared__ float share[kStepSplits];
   const long row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
   const float* stat = p.stat + row * p.splits * 2;
-  float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, stat[2 * s]);
-  float sum = 0.f;
-  for (int s = 0; s < p.splits; ++s) sum += stat[2 * s + 1] * __builtin_amdgcn_exp2f(stat[2 * s] - top);
-  const float inv = 1.f / sum;
-  for (int d = threadIdx.x; d < p.D; d += 64) {
-    float x = 0.f;
-    for (int s = 0; s < p.splits; ++s)
-      x += p.part[(row * p.splits + s) * p.D + d] * __builtin_amdgcn_exp2f(stat[2 * s] - top);
-    ((__bf16*)p.o)[row * p.D + d] = to16<E>(x * inv);
+  // both waves take the maximum and the sum, a split a lane
+  float top = -INFINITY, sum = 0.f;
+  for (int s = lane; s < p.splits; s += 64) top = fmaxf(top, stat[2 * s]);
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k, 64));
+  for (int s = lane; s < p.splits; s += 64) {
+    const float f = __builtin_amdgcn_exp2f(stat[2 * s] - top);
+    if (threadIdx.x < 64) share[s] = f;
+    sum += stat[2 * s + 1] * f;
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k, 64);
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < p.D) {
+    const float* part = p.part + row * p.splits * p.D + d;
+    float x = 0.f, y[8];
+    for (int s = 0; s < p.splits; s += 8) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) y[u] = s + u < p.splits ? part[(s + u) * p.D] * share[s + u] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x += y[u];
+    }
+    ((__bf16*)p.o)[row * p.D + d] = to16<E>(x / sum);
   }
   if (row % p.H == 0 && threadIdx.x == 0) p.counts[row / p.H] = max(p.counts[row / p.H], 0) + 1;
 }
@@ -252,9 +268,9 @@ hipError_t hattn_sliding_step_launch(const SlidingStepArgs& p, int dtype, hipStr
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   const dim3 rows((unsigned)((long)p.B * p.H));
   if (dtype == 1)
-    hipLaunchKernelGGL((sliding_step_join_kernel<_Float16>), rows, dim3(64), 0, stream, p);
+    hipLaunchKernelGGL((sliding_step_join_kernel<_Float16>), rows, dim3(128), 0, stream, p);
   else
-    hipLaunchKernelGGL((sliding_step_join_kernel<__bf16>), rows, dim3(64), 0, stream, p);
+    hipLaunchKernelGGL((sliding_step_join_kernel<__bf16>), rows, dim3(128), 0, stream, p);
   return hipGetLastError();
 }
 

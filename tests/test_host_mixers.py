@@ -159,7 +159,8 @@ def test_sliding_codes(kw, st):
 def test_workspace_queries():
     lib = _lib.load()
     assert lib.hattn_layer_norm_bwd_workspace(4, 16) == 4 * 2 * 16 * 4
-    assert lib.hattn_layer_norm_bwd_workspace(100000, 16) == 512 * 2 * 16 * 4
+    assert lib.hattn_layer_norm_bwd_workspace(100000, 16) == 1024 * 2 * 16 * 4
+    assert lib.hattn_layer_norm_bwd_workspace(100000, 4096) == 512 * 2 * 4096 * 4
     assert lib.hattn_layer_norm_bwd_workspace(0, 16) == 0
     assert lib.hattn_gated_recurrence_segments(256) == 1
     assert lib.hattn_gated_recurrence_segments(257) == 2
