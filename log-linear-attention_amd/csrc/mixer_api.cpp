@@ -103,6 +103,7 @@ int sliding_fill(SlidingArgs& p, const void* q, const void* k, const void* v, co
   p.B = B; p.T = T; p.H = H; p.G = G; p.D = D;
   p.W = std::min(window, T);  // a window of T keys holds every earlier one
   p.S = std::min(sinks, T);
+  p.narrow = p.W + p.S <= kNarrow;
   p.scale = scale;
   p.scale2 = scale * kLog2e;
   return HATTN_OK;

@@ -12,11 +12,13 @@ struct SlidingArgs {
   const int* lengths;                 // [B] or NULL
   long qb, qt, qh, kb, kt, kh, vb, vt, vh;  // strides of q, k, v in elements
   int B, T, H, G, D, W, S;
+  int narrow;                         // W + S <= kNarrow
   float scale, scale2;                // scale, scale * log2(e)
 };
 
 constexpr int kSinkChunk = 1024;  // queries of one partial sum of the sinks' gradients
 constexpr int kMaxSinks = 64;
+constexpr int kNarrow = 64;
 
 // Partial sums a sink's gradient is made of: its near queries, then (chunk, head).
 inline int sliding_sink_slots(int T, int H, int G, int W, int S) {
