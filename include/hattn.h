@@ -688,15 +688,17 @@ int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, c
  * state before and after, each may be NULL (h0: zero); lengths [B] int32 or NULL: row b
  * has lengths[b] tokens (clamped to [0, T]), its later outputs are zero, its later inputs
  * are not used, and ht is the state after its last token.  carry
- * [B, hattn_gated_recurrence_segments(T), D] fp32 (NULL: not kept) is what the backward
- * takes.  Workspace, forward and backward: hattn_gated_recurrence_workspace(B, T, D)
- * bytes, 8-byte aligned, contents on entry ignored.
+ * [B, hattn_gated_recurrence_segments(T, D, dtype_x), D] fp32 (NULL: not kept) is what the
+ * backward takes.  Workspace, forward and backward:
+ * hattn_gated_recurrence_workspace(B, T, D, dtype_x) bytes, 8-byte aligned, contents on entry
+ * ignored.  Where x has 16 bits and D is even, x, g, o and the gradients are aligned to two of
+ * their elements.
  *
  * Workgroups wait, with a bounded poll, for the states of earlier segments; a wait that
  * gives up (two calls that overlap on one workspace) gives NaN, not plausible numbers.
  */
-int hattn_gated_recurrence_segments(int T);
-size_t hattn_gated_recurrence_workspace(int B, int T, int D);
+int hattn_gated_recurrence_segments(int T, int D, int dtype_x);
+size_t hattn_gated_recurrence_workspace(int B, int T, int D, int dtype_x);
 int hattn_gated_recurrence_fwd(const void* x, const void* g, const float* h0, const int* lengths,
                                void* o, float* ht, float* carry, int B, int T, int D, int dtype_x,
                                int dtype_g, void* ws, size_t ws_bytes, void* stream);

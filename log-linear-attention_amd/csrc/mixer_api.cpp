@@ -41,20 +41,47 @@ int norm_checks(long long rows, int n, int dtype_x, int dtype_r, int dtype_w, bo
   return HATTN_OK;
 }
 
+// 16-bit channels go two to a lane where D is even.
+RecurrenceArgs recurrence_shape(int B, int T, int D, int dtype_x) {
+  RecurrenceArgs p{};
+  p.B = B; p.T = T; p.D = D;
+  p.vec = dtype_x != HATTN_FP32 && D % 2 == 0 ? 2 : 1;
+  p.strips = (D + 64 * p.vec - 1) / (64 * p.vec);
+  const int tokens = hattn_recurrence_segment(p.vec);
+  p.nseg = (T - 1) / tokens + 1;
+  return p;
+}
+
 int recurrence_checks(int B, int T, int D, int dtype_x, int dtype_g) {
   if (B <= 0 || T <= 0 || D <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (int st = check_dtype(dtype_x, "x")) return st;
   if (dtype_g != dtype_x && dtype_g != HATTN_FP32)
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "g of dtype code %d with x of %d", dtype_g, dtype_x);
-  const long long strips = (D + 63) / 64;
-  if (B * strips * hattn_recurrence_segments(T) >= (1LL << 31))
+  const RecurrenceArgs p = recurrence_shape(B, T, D, dtype_x);
+  if ((long long)p.B * p.strips * p.nseg >= (1LL << 31))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d D=%d: 2^31 segments", B, T, D);
   return HATTN_OK;
 }
 
-size_t recurrence_ws(int B, int T, int D) {
-  const size_t nseg = hattn_recurrence_segments(T);
-  return nseg > 1 ? nseg * B * ((D + 63) / 64) * 64 * 8 : 0;
+size_t recurrence_ws(const RecurrenceArgs& p) {
+  return p.nseg > 1 ? (size_t)p.nseg * p.B * p.strips * 64 * p.vec * 8 : 0;
+}
+
+// The scan's tensors: rows of vec channels are read at once.
+int recurrence_tensors(const RecurrenceArgs& p, std::initializer_list<const void*> xs,
+                       std::initializer_list<const void*> gs, int dtype_x, int dtype_g,
+                       size_t ws_bytes) {
+  const auto bytes = [](int code) { return code == HATTN_FP32 ? 4 : 2; };
+  for (const void* q : xs)
+    if (!q) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  for (const void* q : gs)
+    if (!q) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  if (!aligned(xs, bytes(dtype_x) * p.vec) || !aligned(gs, bytes(dtype_g) * p.vec))
+    return fail(HATTN_ERR_VALUE, "tensor not aligned to %d of its elements", p.vec);
+  const size_t need = recurrence_ws(p);
+  if (need > 0 && (!p.ws || ws_bytes < need || !aligned({p.ws}, 8)))
+    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
+  return HATTN_OK;
 }
 
 int sliding_checks(int B, int H, int G, int D, int window, int sinks, float scale, int dtype) {
@@ -158,24 +185,23 @@ int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, c
                    "hattn_layer_norm_bwd launch");
 }
 
-int hattn_gated_recurrence_segments(int T) { return T > 0 ? hattn_recurrence_segments(T) : 0; }
+int hattn_gated_recurrence_segments(int T, int D, int dtype_x) {
+  return recurrence_checks(1, T, D, dtype_x, dtype_x) == HATTN_OK
+             ? recurrence_shape(1, T, D, dtype_x).nseg : 0;
+}
 
-size_t hattn_gated_recurrence_workspace(int B, int T, int D) {
-  if (recurrence_checks(B, T, D, HATTN_FP32, HATTN_FP32) != HATTN_OK) return 0;
-  return recurrence_ws(B, T, D);
+size_t hattn_gated_recurrence_workspace(int B, int T, int D, int dtype_x) {
+  return recurrence_checks(B, T, D, dtype_x, dtype_x) == HATTN_OK
+             ? recurrence_ws(recurrence_shape(B, T, D, dtype_x)) : 0;
 }
 
 int hattn_gated_recurrence_fwd(const void* x, const void* g, const float* h0, const int* lengths,
                                void* o, float* ht, float* carry, int B, int T, int D, int dtype_x,
                                int dtype_g, void* ws, size_t ws_bytes, void* stream) {
   if (int st = recurrence_checks(B, T, D, dtype_x, dtype_g)) return st;
-  if (!x || !g || !o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
-  const size_t need = recurrence_ws(B, T, D);
-  if (need > 0 && (!ws || ws_bytes < need || !aligned({ws}, 8)))
-    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
-  RecurrenceArgs p{};
+  RecurrenceArgs p = recurrence_shape(B, T, D, dtype_x);
   p.x = x; p.g = g; p.h0 = h0; p.lengths = lengths; p.o = o; p.ht = ht; p.carry = carry; p.ws = ws;
-  p.B = B; p.T = T; p.D = D; p.strips = (D + 63) / 64; p.nseg = hattn_recurrence_segments(T);
+  if (int st = recurrence_tensors(p, {x, o}, {g}, dtype_x, dtype_g, ws_bytes)) return st;
   return check_hip(hattn_recurrence_launch(0, p, dtype_x, dtype_g, (hipStream_t)stream),
                    "hattn_gated_recurrence_fwd launch");
 }
@@ -185,14 +211,11 @@ int hattn_gated_recurrence_bwd(const void* x, const void* g, const float* carry,
                                void* dg, float* dh0, int B, int T, int D, int dtype_x, int dtype_g,
                                void* ws, size_t ws_bytes, void* stream) {
   if (int st = recurrence_checks(B, T, D, dtype_x, dtype_g)) return st;
-  if (!x || !g || !carry || !dout || !dx || !dg) return fail(HATTN_ERR_VALUE, "null tensor pointer");
-  const size_t need = recurrence_ws(B, T, D);
-  if (need > 0 && (!ws || ws_bytes < need || !aligned({ws}, 8)))
-    return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
-  RecurrenceArgs p{};
+  if (!carry) return fail(HATTN_ERR_VALUE, "null tensor pointer");
+  RecurrenceArgs p = recurrence_shape(B, T, D, dtype_x);
   p.x = x; p.g = g; p.go = dout; p.ght = dht; p.lengths = lengths; p.dx = dx; p.dg = dg;
   p.dh0 = dh0; p.carry = const_cast<float*>(carry); p.ws = ws;
-  p.B = B; p.T = T; p.D = D; p.strips = (D + 63) / 64; p.nseg = hattn_recurrence_segments(T);
+  if (int st = recurrence_tensors(p, {x, dout, dx}, {g, dg}, dtype_x, dtype_g, ws_bytes)) return st;
   return check_hip(hattn_recurrence_launch(1, p, dtype_x, dtype_g, (hipStream_t)stream),
                    "hattn_gated_recurrence_bwd launch");
 }

@@ -6,12 +6,16 @@
 // Both directions compose affine maps h -> A h + X, which is associative:
 //   (A2, X2) o (A1, X1) = (A2 A1, A2 X1 + X2).
 //
-// A lane owns one channel, a wave 32 tokens of 64 channels held in registers, a
-// workgroup 256 tokens (a segment).  Inside the workgroup the waves' maps meet in
+// A lane owns one channel in 32 bits, or two next to each other in 16 bits (where D is even):
+// a wave reads rows of 256 bytes (rows of 128 took 103 and not 93 us forward, 150 and not
+// 133 backward, at B 4, T 8192, D 2048).  A wave holds 32 or 16 tokens in registers, a
+// workgroup eight times as many (a segment); registers are held to 128, so that a second
+// workgroup on the CU loads and stores while the first waits (133 and not 162 us backward).  Inside the workgroup the waves' maps meet in
 // LDS; between the segments of a channel the workgroup publishes its map in a word
 // {A, X} and then walks back over the words before it until one has A = 0.  A
 // segment whose state is known replaces its word by {0, h}, so the walk is short, and
-// the data is read once and written once: bound by the bytes.
+// the data is read once and written once: bound by the bytes (forward 4.3 TB/s and backward
+// 5.0 at the shape above in bf16, forward 4.9 at B 1, T 131072, D 1024 in fp32).
 //
 // A word is 64 bits wide and is written and read by one atomic access of device
 // scope, so it is its own flag: kEmpty (a NaN pattern that publish() never writes)
@@ -23,9 +27,9 @@
 
 namespace hattn {
 
-constexpr int kTok = 32;                 // tokens a wave
 constexpr int kWaves = 8;                // waves a workgroup
-constexpr int kSeg = kTok * kWaves;      // tokens a segment
+template <int VEC>
+constexpr int kTok = 32 / VEC;           // tokens a wave
 constexpr unsigned long long kEmpty = ~0ull;
 constexpr int kSpins = 1 << 20;          // rounds of a wait, about a second
 
@@ -99,13 +103,14 @@ __global__ void fill_empty_kernel(unsigned long long* w, long n) {
     w[i] = kEmpty;
 }
 
-// blockIdx.x = segment * units + unit, unit = batch * strips + strip of 64 channels:
+// blockIdx.x = segment * units + unit, unit = batch * strips + strip of 64 lanes:
 // every unit's first segment is dispatched first.
 struct Place {
   int b, d, seg, len;
   long unit;
-  bool live;
+  bool live;  // all of a lane's channels are there or none
 };
+template <int VEC>
 __device__ __forceinline__ Place place(const RecurrenceArgs& p, bool backward) {
   Place at;
   const int units = p.B * p.strips;
@@ -113,154 +118,213 @@ __device__ __forceinline__ Place place(const RecurrenceArgs& p, bool backward) {
   at.seg = backward ? p.nseg - 1 - s : s;
   at.unit = u;
   at.b = u / p.strips;
-  at.d = (u % p.strips) * 64 + (threadIdx.x & 63);
+  at.d = ((u % p.strips) * 64 + (threadIdx.x & 63)) * VEC;
   at.live = at.d < p.D;
   at.len = p.lengths ? min(max(p.lengths[at.b], 0), p.T) : p.T;
   return at;
 }
 
-template <typename TX, typename TG>
+// VEC values of a row, and their store.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&out)[VEC]) {
+  typedef T TV __attribute__((ext_vector_type(VEC)));
+  if constexpr (VEC == 1) {
+    out[0] = to_f32<T>(p[0]);
+  } else {
+    const TV x = *(const TV*)p;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = to_f32<T>(x[e]);
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
+  typedef T TV __attribute__((ext_vector_type(VEC)));
+  if constexpr (VEC == 1) {
+    p[0] = from_f32<T>(x[0]);
+  } else {
+    TV y;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) y[e] = from_f32<T>(x[e]);
+    *(TV*)p = y;
+  }
+}
+
+template <typename TX, typename TG, int VEC>
 __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(RecurrenceArgs p) {
-  __shared__ Map maps[kWaves][64];
-  __shared__ float enter[64];
-  const Place at = place(p, false);
+  constexpr int TOK = kTok<VEC>;
+  __shared__ Map maps[kWaves][VEC][64];
+  __shared__ float enter[VEC][64];
+  const Place at = place<VEC>(p, false);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t0 = at.seg * kSeg + wave * kTok;
-  const long base = (long)at.b * p.T * p.D;
+  const int t0 = (at.seg * kWaves + wave) * TOK;
+  const int d = at.live ? at.d : 0;
+  const long base = (long)at.b * p.T * p.D + d;
   const TX* x = (const TX*)p.x + base;
   const TG* g = (const TG*)p.g + base;
-  const int d = at.live ? at.d : p.D - 1;
 
-  float a[kTok], v[kTok];
+  float a[TOK][VEC], v[TOK][VEC];
   if (t0 < p.T) {
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
+    for (int i = 0; i < TOK; ++i) {
       // rows past the end read the last one; what they read is not used
-      const long row = (long)min(t0 + i, p.T - 1) * p.D + d;
-      v[i] = to_f32<TX>(x[row]);
-      a[i] = to_f32<TG>(g[row]);
+      const long row = (long)min(t0 + i, p.T - 1) * p.D;
+      load_vec<TX, VEC>(x + row, v[i]);
+      load_vec<TG, VEC>(g + row, a[i]);
     }
   }
-  float A = 1.f, X = 0.f;
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    const bool in = t0 + i < at.len;
-    a[i] = in ? fexp(a[i]) : 1.f;
-    v[i] = in ? v[i] : 0.f;
-    X = a[i] * X + v[i];
-    A *= a[i];
+  for (int e = 0; e < VEC; ++e) {
+    float A = 1.f, X = 0.f;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const bool in = t0 + i < at.len;
+      a[i][e] = in ? fexp(a[i][e]) : 1.f;
+      v[i][e] = in ? v[i][e] : 0.f;
+      X = a[i][e] * X + v[i][e];
+      A *= a[i][e];
+    }
+    maps[wave][e][lane] = Map{A, X};
   }
-  maps[wave][lane] = Map{A, X};
   __syncthreads();
-  if (wave == 0) {
-    Map m = maps[0][lane];
+  // the first waves join the maps, one for each of a lane's channels
+  if (wave < VEC) {
+    const int e = wave;
+    Map m = maps[0][e][lane];
 #pragma unroll
     for (int k = 1; k < kWaves; ++k) {
-      const Map n = maps[k][lane];
+      const Map n = maps[k][e][lane];
       m = Map{n.A * m.A, n.A * m.X + n.X};
     }
-    const float h0 = p.h0 && at.live ? p.h0[(long)at.b * p.D + d] : 0.f;
-    const long stride = (long)p.B * p.strips * 64;
-    unsigned long long* w = (unsigned long long*)p.ws + at.seg * stride + at.unit * 64 + lane;
+    const float h0 = p.h0 && at.live ? p.h0[(long)at.b * p.D + d + e] : 0.f;
+    const long stride = (long)p.B * p.strips * 64 * VEC;
+    unsigned long long* w =
+        (unsigned long long*)p.ws + at.seg * stride + (at.unit * VEC + e) * 64 + lane;
     const bool last = at.seg == p.nseg - 1;
     if (at.live && !last && at.seg > 0) publish(w, m.A, m.X);
     const float h = look_back(w - stride, -stride, at.seg, h0, at.live);
     // as apply(): A = 0 ends a walk, so nothing before such a segment reaches past it
     const float out = m.A == 0.f ? m.X : m.A * h + m.X;
     if (at.live && !last) publish(w, 0.f, out);
-    if (at.live && last && p.ht) p.ht[(long)at.b * p.D + d] = out;
-    if (at.live && p.carry) p.carry[((long)at.b * p.nseg + at.seg) * p.D + d] = h;
-    enter[lane] = h;
+    if (at.live && last && p.ht) p.ht[(long)at.b * p.D + d + e] = out;
+    if (at.live && p.carry) p.carry[((long)at.b * p.nseg + at.seg) * p.D + d + e] = h;
+    enter[e][lane] = h;
   }
   __syncthreads();
-  float h = enter[lane];
-  for (int k = 0; k < wave; ++k) h = maps[k][lane].A * h + maps[k][lane].X;
+  float h[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    h[e] = enter[e][lane];
+    for (int k = 0; k < wave; ++k) h[e] = maps[k][e][lane].A * h[e] + maps[k][e][lane].X;
+  }
   TX* o = (TX*)p.o + base;
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    h = a[i] * h + v[i];
-    if (at.live && t0 + i < p.T) o[(long)(t0 + i) * p.D + d] = from_f32<TX>(t0 + i < at.len ? h : 0.f);
+  for (int i = 0; i < TOK; ++i) {
+    float y[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      h[e] = a[i][e] * h[e] + v[i][e];
+      y[e] = t0 + i < at.len ? h[e] : 0.f;
+    }
+    if (at.live && t0 + i < p.T) store_vec<TX, VEC>(o + (long)(t0 + i) * p.D, y);
   }
 }
 
-template <typename TX, typename TG>
-__global__ __launch_bounds__(64 * kWaves) void recurrence_bwd_kernel(RecurrenceArgs p) {
-  __shared__ Map fwd[kWaves][64], bwd[kWaves][64];
-  __shared__ float enter[64];
-  const Place at = place(p, true);
+template <typename TX, typename TG, int VEC>
+__global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(RecurrenceArgs p) {
+  constexpr int TOK = kTok<VEC>;
+  __shared__ Map fwd[kWaves][VEC][64], bwd[kWaves][VEC][64];
+  __shared__ float enter[VEC][64];
+  const Place at = place<VEC>(p, true);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t0 = at.seg * kSeg + wave * kTok;
-  const long base = (long)at.b * p.T * p.D;
+  const int t0 = (at.seg * kWaves + wave) * TOK;
+  const int d = at.live ? at.d : 0;
+  const long base = (long)at.b * p.T * p.D + d;
   const TX *x = (const TX*)p.x + base, *go = (const TX*)p.go + base;
   const TG* g = (const TG*)p.g + base;
-  const int d = at.live ? at.d : p.D - 1;
 
-  float a[kTok], v[kTok], q[kTok];
+  float a[TOK][VEC], v[TOK][VEC], q[TOK][VEC];
   if (t0 < p.T) {
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const long row = (long)min(t0 + i, p.T - 1) * p.D + d;
-      a[i] = to_f32<TG>(g[row]);
-      q[i] = to_f32<TX>(go[row]);
-      v[i] = to_f32<TX>(x[row]);
+    for (int i = 0; i < TOK; ++i) {
+      const long row = (long)min(t0 + i, p.T - 1) * p.D;
+      load_vec<TG, VEC>(g + row, a[i]);
+      load_vec<TX, VEC>(go + row, q[i]);
+      load_vec<TX, VEC>(x + row, v[i]);
     }
   }
-  float A = 1.f, X = 0.f, E = 0.f;
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    const bool in = t0 + i < at.len;
-    a[i] = in ? fexp(a[i]) : 1.f;
-    v[i] = in ? v[i] : 0.f;
-    q[i] = in ? q[i] : 0.f;
-    X = a[i] * X + v[i];
-    A *= a[i];
+  for (int e = 0; e < VEC; ++e) {
+    float A = 1.f, X = 0.f, E = 0.f;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const bool in = t0 + i < at.len;
+      a[i][e] = in ? fexp(a[i][e]) : 1.f;
+      v[i][e] = in ? v[i][e] : 0.f;
+      q[i][e] = in ? q[i][e] : 0.f;
+      X = a[i][e] * X + v[i][e];
+      A *= a[i][e];
+    }
+#pragma unroll
+    for (int i = TOK - 1; i >= 0; --i) E = a[i][e] * (q[i][e] + E);
+    fwd[wave][e][lane] = Map{A, X};
+    bwd[wave][e][lane] = Map{A, E};
   }
-#pragma unroll
-  for (int i = kTok - 1; i >= 0; --i) E = a[i] * (q[i] + E);
-  fwd[wave][lane] = Map{A, X};
-  bwd[wave][lane] = Map{A, E};
   __syncthreads();
-  if (wave == 0) {
-    Map m = bwd[kWaves - 1][lane];
+  if (wave < VEC) {
+    const int e = wave;
+    Map m = bwd[kWaves - 1][e][lane];
 #pragma unroll
     for (int k = kWaves - 2; k >= 0; --k) {
-      const Map n = bwd[k][lane];
+      const Map n = bwd[k][e][lane];
       m = Map{n.A * m.A, n.A * m.X + n.X};
     }
-    const float end = p.ght && at.live ? p.ght[(long)at.b * p.D + d] : 0.f;
-    const long stride = (long)p.B * p.strips * 64;
-    unsigned long long* w = (unsigned long long*)p.ws + at.seg * stride + at.unit * 64 + lane;
+    const float end = p.ght && at.live ? p.ght[(long)at.b * p.D + d + e] : 0.f;
+    const long stride = (long)p.B * p.strips * 64 * VEC;
+    unsigned long long* w =
+        (unsigned long long*)p.ws + at.seg * stride + (at.unit * VEC + e) * 64 + lane;
     const int after = p.nseg - 1 - at.seg;
     if (at.live && after > 0 && at.seg > 0) publish(w, m.A, m.X);
-    const float e = look_back(w + stride, stride, after, end, at.live);
-    const float out = m.A == 0.f ? m.X : m.A * e + m.X;
+    const float in = look_back(w + stride, stride, after, end, at.live);
+    const float out = m.A == 0.f ? m.X : m.A * in + m.X;
     if (at.live && at.seg > 0) publish(w, 0.f, out);
-    if (at.live && at.seg == 0 && p.dh0) p.dh0[(long)at.b * p.D + d] = out;
-    enter[lane] = e;
+    if (at.live && at.seg == 0 && p.dh0) p.dh0[(long)at.b * p.D + d + e] = out;
+    enter[e][lane] = in;
   }
-  // the state that enters this wave's tokens, while wave 0 looks ahead
-  float h = p.carry[((long)at.b * p.nseg + at.seg) * p.D + d];
-  for (int k = 0; k < wave; ++k) h = fwd[k][lane].A * h + fwd[k][lane].X;
+  // the state that enters this wave's tokens, while the first waves look ahead
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    const float was = h;
-    h = a[i] * h + v[i];
-    v[i] = was;
+  for (int e = 0; e < VEC; ++e) {
+    float h = p.carry[((long)at.b * p.nseg + at.seg) * p.D + d + e];
+    for (int k = 0; k < wave; ++k) h = fwd[k][e][lane].A * h + fwd[k][e][lane].X;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      const float was = h;
+      h = a[i][e] * h + v[i][e];
+      v[i][e] = was;
+    }
   }
   __syncthreads();
-  float e = enter[lane];
-  for (int k = kWaves - 1; k > wave; --k) e = bwd[k][lane].A * e + bwd[k][lane].X;
+  float s[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    s[e] = enter[e][lane];
+    for (int k = kWaves - 1; k > wave; --k) s[e] = bwd[k][e][lane].A * s[e] + bwd[k][e][lane].X;
+  }
   TX* dx = (TX*)p.dx + base;
   TG* dg = (TG*)p.dg + base;
 #pragma unroll
-  for (int i = kTok - 1; i >= 0; --i) {
-    const float dh = q[i] + e;
-    e = a[i] * dh;
+  for (int i = TOK - 1; i >= 0; --i) {
+    const bool in = t0 + i < at.len;
+    float y[VEC], z[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float dh = q[i][e] + s[e];
+      s[e] = a[i][e] * dh;
+      y[e] = in ? dh : 0.f;
+      z[e] = in ? s[e] * v[i][e] : 0.f;
+    }
     if (at.live && t0 + i < p.T) {
-      const long row = (long)(t0 + i) * p.D + d;
-      const bool in = t0 + i < at.len;
-      dx[row] = from_f32<TX>(in ? dh : 0.f);
-      dg[row] = from_f32<TG>(in ? e * v[i] : 0.f);
+      store_vec<TX, VEC>(dx + (long)(t0 + i) * p.D, y);
+      store_vec<TG, VEC>(dg + (long)(t0 + i) * p.D, z);
     }
   }
 }
@@ -277,6 +341,23 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(float* __restrict_
   o[i] = from_f32<TX>(y);
 }
 
+template <typename TX, typename TG, int VEC>
+static hipError_t launch_scan(int what, const RecurrenceArgs& p, hipStream_t stream) {
+  const long units = (long)p.B * p.strips;
+  if (p.nseg > 1) {
+    const long n = units * 64 * VEC * p.nseg;
+    const long want = (n + 1023) / 1024;
+    hipLaunchKernelGGL(fill_empty_kernel, dim3((unsigned)(want < 1024 ? want : 1024)), dim3(256), 0,
+                       stream, (unsigned long long*)p.ws, n);
+  }
+  const dim3 grid((unsigned)(units * p.nseg)), block(64 * kWaves);
+  if (what == 0)
+    hipLaunchKernelGGL((recurrence_fwd_kernel<TX, TG, VEC>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((recurrence_bwd_kernel<TX, TG, VEC>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
 template <typename TX, typename TG>
 static hipError_t launch(int what, const RecurrenceArgs& p, hipStream_t stream) {
   if (what == 2) {
@@ -285,24 +366,14 @@ static hipError_t launch(int what, const RecurrenceArgs& p, hipStream_t stream) 
                        dim3(256), 0, stream, p.ht, (const TX*)p.x, (const TG*)p.g, (TX*)p.o, n);
     return hipGetLastError();
   }
-  const long units = (long)p.B * p.strips;
-  if (p.nseg > 1) {
-    const long n = units * 64 * p.nseg;
-    const long want = (n + 1023) / 1024;
-    hipLaunchKernelGGL(fill_empty_kernel, dim3((unsigned)(want < 1024 ? want : 1024)), dim3(256), 0,
-                       stream, (unsigned long long*)p.ws, n);
-  }
-  const dim3 grid((unsigned)(units * p.nseg));
-  if (what == 0)
-    hipLaunchKernelGGL((recurrence_fwd_kernel<TX, TG>), grid, dim3(64 * kWaves), 0, stream, p);
-  else
-    hipLaunchKernelGGL((recurrence_bwd_kernel<TX, TG>), grid, dim3(64 * kWaves), 0, stream, p);
-  return hipGetLastError();
+  if constexpr (sizeof(TX) == 2)
+    if (p.vec == 2) return launch_scan<TX, TG, 2>(what, p, stream);
+  return launch_scan<TX, TG, 1>(what, p, stream);
 }
 
 }  // namespace hattn
 
-int hattn_recurrence_segments(int T) { return (T + hattn::kSeg - 1) / hattn::kSeg; }
+int hattn_recurrence_segment(int vec) { return (32 / vec) * hattn::kWaves; }
 
 // what: 0 forward, 1 backward, 2 step
 hipError_t hattn_recurrence_launch(int what, const RecurrenceArgs& p, int dtype_x, int dtype_g,

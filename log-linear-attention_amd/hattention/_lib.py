@@ -84,8 +84,8 @@ SIGNATURES = [
     ("hattn_layer_norm_fwd", _I, [_P] * 8 + [_LL, _I, ctypes.c_float] + [_I] * 3 + [_P]),
     ("hattn_layer_norm_bwd_workspace", _S, [_LL, _I]),
     ("hattn_layer_norm_bwd", _I, [_P] * 10 + [_LL, _I] + [_I] * 3 + [_P, _S, _P]),
-    ("hattn_gated_recurrence_segments", _I, [_I]),
-    ("hattn_gated_recurrence_workspace", _S, [_I] * 3),
+    ("hattn_gated_recurrence_segments", _I, [_I] * 3),
+    ("hattn_gated_recurrence_workspace", _S, [_I] * 4),
     ("hattn_gated_recurrence_fwd", _I, [_P] * 7 + [_I] * 5 + [_P, _S, _P]),
     ("hattn_gated_recurrence_bwd", _I, [_P] * 9 + [_I] * 5 + [_P, _S, _P]),
     ("hattn_gated_recurrence_step", _I, [_P] * 4 + [_I] * 4 + [_P]),

@@ -28,25 +28,32 @@ def check_lengths(lengths, B: int, dev) -> Optional[torch.Tensor]:
     return lengths.contiguous()
 
 
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and starting on 8 bytes: the kernels read two channels at a time."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 8 == 0 else t.clone()
+
+
 def _forward(x, g, h0, lengths, final, keep):
     """(o, ht or None, carry or None)."""
     B, T, D = x.shape
     dev = x.device
     lib = _lib.load()
+    code = _lib.dtype_code(x)
     o = torch.empty(B, T, D, dtype=x.dtype, device=dev)
     ht = torch.empty(B, D, dtype=torch.float32, device=dev) if final else None
-    carry = torch.empty(B, lib.hattn_gated_recurrence_segments(T), D, dtype=torch.float32,
+    carry = torch.empty(B, lib.hattn_gated_recurrence_segments(T, D, code), D, dtype=torch.float32,
                         device=dev) if keep else None
-    ws, ws_ptr, ws_bytes = _lib.workspace(lib.hattn_gated_recurrence_workspace(B, T, D), dev)
+    ws, ws_ptr, ws_bytes = _lib.workspace(lib.hattn_gated_recurrence_workspace(B, T, D, code), dev)
     _lib.launch(dev, lib.hattn_gated_recurrence_fwd, x.data_ptr(), g.data_ptr(), _lib.ptr(h0),
                 _lib.ptr(lengths), o.data_ptr(), _lib.ptr(ht), _lib.ptr(carry), B, T, D,
-                _lib.dtype_code(x), _lib.dtype_code(g), ws_ptr, ws_bytes)
+                code, _lib.dtype_code(g), ws_ptr, ws_bytes)
     return o, ht, carry
 
 
 class GatedRecurrenceFunction(torch.autograd.Function):
     """(o, ht) of :func:`gated_linear_recurrence`.  The states that enter each segment are
-    kept for the backward (4 bytes for 256 tokens of a channel)."""
+    kept for the backward (4 bytes for 128 or 256 tokens of a channel)."""
 
     @staticmethod
     def forward(ctx, x, g, h0, lengths, final):
@@ -65,16 +72,18 @@ class GatedRecurrenceFunction(torch.autograd.Function):
             if dht is None:
                 return None, None, None, None, None
             do = torch.zeros_like(x)
-        do = do.contiguous()
+        do = _aligned(do)
         dht = dht.contiguous() if dht is not None else None
         dx, dg = torch.empty_like(x), torch.empty_like(g)
         dh0 = torch.empty(B, D, dtype=torch.float32, device=dev) \
             if ctx.needs_input_grad[2] else None
         lib = _lib.load()
-        ws, ws_ptr, ws_bytes = _lib.workspace(lib.hattn_gated_recurrence_workspace(B, T, D), dev)
+        code = _lib.dtype_code(x)
+        ws, ws_ptr, ws_bytes = _lib.workspace(
+            lib.hattn_gated_recurrence_workspace(B, T, D, code), dev)
         _lib.launch(dev, lib.hattn_gated_recurrence_bwd, x.data_ptr(), g.data_ptr(),
                     carry.data_ptr(), _lib.ptr(lengths), do.data_ptr(), _lib.ptr(dht),
-                    dx.data_ptr(), dg.data_ptr(), _lib.ptr(dh0), B, T, D, _lib.dtype_code(x),
+                    dx.data_ptr(), dg.data_ptr(), _lib.ptr(dh0), B, T, D, code,
                     _lib.dtype_code(g), ws_ptr, ws_bytes)
         need = ctx.needs_input_grad
         return dx if need[0] else None, dg if need[1] else None, dh0, None, None
@@ -111,7 +120,7 @@ def gated_linear_recurrence(x: torch.Tensor, g: torch.Tensor,
         raise ValueError(f"initial_state must be [{B}, {D}]")
     dev = _lib.require_device(x, g, initial_state)
     lengths = check_lengths(lengths, B, dev)
-    x, g = x.contiguous(), g.contiguous()
+    x, g = _aligned(x), _aligned(g)
     h0 = initial_state.float().contiguous() if initial_state is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad
                                     or (h0 is not None and h0.requires_grad)):

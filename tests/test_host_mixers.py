@@ -162,11 +162,15 @@ def test_workspace_queries():
     assert lib.hattn_layer_norm_bwd_workspace(100000, 16) == 1024 * 2 * 16 * 4
     assert lib.hattn_layer_norm_bwd_workspace(100000, 4096) == 512 * 2 * 4096 * 4
     assert lib.hattn_layer_norm_bwd_workspace(0, 16) == 0
-    assert lib.hattn_gated_recurrence_segments(256) == 1
-    assert lib.hattn_gated_recurrence_segments(257) == 2
-    assert lib.hattn_gated_recurrence_workspace(2, 256, 100) == 0
-    assert lib.hattn_gated_recurrence_workspace(2, 257, 100) == 2 * 2 * 128 * 8
-    assert lib.hattn_gated_recurrence_workspace(0, 257, 100) == 0
+    # fp32, or an odd number of channels: 256 tokens a segment, strips of 64; else 128 and 128
+    assert lib.hattn_gated_recurrence_segments(256, 100, 2) == 1
+    assert lib.hattn_gated_recurrence_segments(257, 101, 0) == 2
+    assert lib.hattn_gated_recurrence_segments(256, 100, 1) == 2
+    assert lib.hattn_gated_recurrence_segments(0, 100, 1) == 0
+    assert lib.hattn_gated_recurrence_workspace(2, 256, 100, 2) == 0
+    assert lib.hattn_gated_recurrence_workspace(2, 257, 100, 2) == 2 * 2 * 128 * 8
+    assert lib.hattn_gated_recurrence_workspace(2, 257, 130, 0) == 3 * 2 * 256 * 8
+    assert lib.hattn_gated_recurrence_workspace(0, 257, 100, 2) == 0
     # delta, and the sinks' partial sums: the near one and a (chunk of 1024, head) each
     delta = 2 * 4 * 3000 * 4
     assert lib.hattn_sliding_bwd_workspace(2, 3000, 4, 2, 64, 3000, 8) == delta
