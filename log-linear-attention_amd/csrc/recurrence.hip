@@ -10,12 +10,14 @@
 // a wave reads rows of 256 bytes (rows of 128 took 103 and not 93 us forward, 150 and not
 // 133 backward, at B 4, T 8192, D 2048).  A wave holds 32 or 16 tokens in registers, a
 // workgroup eight times as many (a segment); registers are held to 128, so that a second
-// workgroup on the CU loads and stores while the first waits (133 and not 162 us backward).  Inside the workgroup the waves' maps meet in
-// LDS; between the segments of a channel the workgroup publishes its map in a word
-// {A, X} and then walks back over the words before it until one has A = 0.  A
-// segment whose state is known replaces its word by {0, h}, so the walk is short, and
-// the data is read once and written once: bound by the bytes (forward 4.3 TB/s and backward
-// 5.0 at the shape above in bf16, forward 4.9 at B 1, T 131072, D 1024 in fp32).
+// workgroup on the CU loads and stores while the first waits (133 and not 162 us backward).
+//
+// Inside the workgroup the waves' maps meet in LDS; between the segments of a channel the
+// workgroup publishes its map in a word {A, X} and then walks back over the words before it
+// until one has A = 0.  A segment whose state is known replaces its word by {0, h}, so the
+// walk is short, and the data is read once and written once: bound by the bytes (forward
+// 4.3 TB/s and backward 5.0 at the shape above in bf16, forward 4.9 at B 1, T 131072, D 1024
+// in fp32).
 //
 // A word is 64 bits wide and is written and read by one atomic access of device
 // scope, so it is its own flag: kEmpty (a NaN pattern that publish() never writes)
