@@ -56,6 +56,28 @@ __device__ __forceinline__ void store_row(T* p, const float (&x)[VEC]) {
   }
 }
 
+// VEC elements of a row as they lie in memory, so that a load can be in flight over other work.
+template <typename T, int VEC>
+struct RawRow {
+  T x[VEC];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) {
+      x[0] = p[0];
+    } else if constexpr (sizeof(T) == 2) {
+      const uint4 r = *(const uint4*)p;
+      __builtin_memcpy(x, &r, 16);
+    } else {
+      const floatx4 a = ((const floatx4*)p)[0], b = ((const floatx4*)p)[1];
+      __builtin_memcpy(x, &a, 16);
+      __builtin_memcpy(x + 4, &b, 16);
+    }
+  }
+  __device__ __forceinline__ void get(float (&out)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = to_f32<T>(x[i]);
+  }
+};
+
 // VEC elements of a parameter from element `at` on, x in each where there is none.
 template <int VEC>
 __device__ __forceinline__ void load_params(const void* p, int dtype, int at, int n, float x,
