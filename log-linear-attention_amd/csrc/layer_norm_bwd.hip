@@ -54,7 +54,10 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
   if (AHEAD && row < rows) fetch(row);
   for (; row < rows; row += step, turn ^= 1) {
     const long base = row * n;
-    if constexpr (!AHEAD) fetch(row);
+    if constexpr (!AHEAD) {
+      mean = mean_in[row];
+      rstd = rstd_in[row];
+    }
     const float mu = mean, rs = rstd;
     float h[CH][VEC], t[CH][VEC], sum[2] = {0.f, 0.f};
     RawRow<TS, VEC> dsn[CH];
@@ -62,9 +65,14 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
     for (int c = 0; c < CH; ++c) {
       const int at = first + c * STEP;
       if (at < n) {
-        sn[c].get(h[c]);
-        dyn[c].get(t[c]);
-        if constexpr (DS) dsn[c].load(ds + base + at);
+        if constexpr (AHEAD) {
+          sn[c].get(h[c]);
+          dyn[c].get(t[c]);
+          if constexpr (DS) dsn[c].load(ds + base + at);
+        } else {
+          load_row<TS, VEC>(s + base + at, h[c]);
+          load_row<TX, VEC>(dy + base + at, t[c]);
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           h[c][i] = (h[c][i] - mu) * rs;
@@ -84,7 +92,8 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
       const int at = first + c * STEP;
       if (at < n) {
         float o[VEC];
-        if constexpr (DS) dsn[c].get(o);
+        if constexpr (DS && AHEAD) dsn[c].get(o);
+        else if constexpr (DS) load_row<TS, VEC>(ds + base + at, o);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           o[i] = (DS ? o[i] : 0.f) + rs * (t[c][i] - c1 - h[c][i] * c2);
