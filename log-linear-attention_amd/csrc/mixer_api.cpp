@@ -18,6 +18,9 @@ namespace {
 
 const float kLog2e = 1.4426950408889634f;
 
+// The attention kernels address the rows of one tile by 32-bit offsets.
+const long long kMaxTokenStride = 1LL << 24;
+
 int check_dtype(int code, const char* what) {
   if (code < HATTN_BF16 || code > HATTN_FP32)
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "%s: dtype code %d", what, code);
@@ -96,17 +99,16 @@ int sliding_checks(int B, int H, int G, int D, int window, int sinks, float scal
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "D=%d is not a multiple of 8 up to 128", D);
   if (dtype != HATTN_BF16 && dtype != HATTN_FP16)
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "dtype code %d (bf16 or fp16 only)", dtype);
+  if ((long long)H * D >= kMaxTokenStride)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "H=%d D=%d: a token of 2^24 elements or more", H, D);
   return HATTN_OK;
 }
-
-const long long kMaxTokenStride = 1LL << 24;
 
 // Strides in elements, batch / token / head of q, k, v: 16-byte rows.
 int stride_checks(const long long* st, int n) {
   for (int i = 0; i < n; ++i)
     if (st[i] % 8 != 0 || st[i] < 0)
       return fail(HATTN_ERR_VALUE, "stride %lld is not a multiple of 8 elements", st[i]);
-  // the rows of one tile are addressed by 32-bit offsets
   for (int i = 1; i < n; i += 3)
     if (st[i] >= kMaxTokenStride)
       return fail(HATTN_ERR_NOT_IMPLEMENTED, "token stride %lld of 2^24 elements or more", st[i]);

@@ -142,7 +142,8 @@ def test_recurrence_codes(B, T, D, dx, dg, st):
 @pytest.mark.parametrize("kw,st", [
     (dict(B=0), VAL), (dict(H=3), VAL), (dict(window=0), VAL), (dict(sinks=-1), VAL),
     (dict(scale=0.0), VAL), (dict(scale=float("nan")), VAL), (dict(sinks=65), NOT),
-    (dict(D=60), NOT), (dict(D=136), NOT), (dict(dtype=2), NOT), (dict(), VAL)])
+    (dict(D=60), NOT), (dict(D=136), NOT), (dict(dtype=2), NOT), (dict(H=2 ** 18, G=2 ** 18), NOT),
+    (dict(), VAL)])
 def test_sliding_codes(kw, st):
     a = dict(B=1, T=4, H=4, G=2, D=64, window=4, sinks=0, scale=0.125, dtype=0)
     a.update(kw)
