@@ -60,6 +60,7 @@ int recurrence_checks(int B, int T, int D, int dtype_x, int dtype_g) {
   if (int st = check_dtype(dtype_x, "x")) return st;
   if (dtype_g != dtype_x && dtype_g != HATTN_FP32)
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "g of dtype code %d with x of %d", dtype_g, dtype_x);
+  if (T > (1 << 30)) return fail(HATTN_ERR_NOT_IMPLEMENTED, "T=%d above 2^30", T);
   const RecurrenceArgs p = recurrence_shape(B, T, D, dtype_x);
   if ((long long)p.B * p.strips * p.nseg >= (1LL << 31))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d D=%d: 2^31 segments", B, T, D);

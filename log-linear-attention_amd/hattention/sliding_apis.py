@@ -7,6 +7,7 @@ kernels are libhattn_hip.so's ``hattn_sliding_fwd`` / ``_bwd`` / ``_cache_fill``
 ``_step``.  No counterpart in the reference.
 """
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -16,6 +17,11 @@ from hattention import _lib
 from hattention.recurrence_apis import check_lengths
 
 MAX_SINKS = 64
+
+
+@functools.lru_cache(maxsize=256)
+def _step_bytes(*sizes) -> int:
+    return _lib.load().hattn_sliding_step_workspace(*sizes)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -129,6 +135,7 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     dev = _lib.require_device(q, k, v)
     lengths = check_lengths(lengths, q.shape[0], dev)
     q, k, v = _rows(q), _rows(k), _rows(v)
+    window = min(window, q.shape[1])  # a window of T keys holds every earlier one
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return SlidingWindowFunction.apply(q, k, v, lengths, window, sinks, scale)
     return _forward(q, k, v, lengths, window, sinks, scale, False)[0]
@@ -203,10 +210,8 @@ def sliding_window_step(state: SlidingState, q: torch.Tensor, k: torch.Tensor, v
     q, k, v = (t if t.is_contiguous() and t.data_ptr() % 16 == 0
                else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
     o = torch.empty_like(q)
-    lib = _lib.load()
-    ws, ws_ptr, ws_bytes = _lib.workspace(
-        lib.hattn_sliding_step_workspace(B, H, G, D, window, sinks), dev)
-    _lib.launch(dev, lib.hattn_sliding_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    ws, ws_ptr, ws_bytes = _lib.workspace(_step_bytes(B, H, G, D, window, sinks), dev)
+    _lib.launch(dev, _lib.load().hattn_sliding_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 kc.data_ptr(), state.v.data_ptr(), state.counts.data_ptr(), o.data_ptr(), B, H, G,
                 D, window, sinks, scale, _lib.dtype_code(q), ws_ptr, ws_bytes)
     return o, state

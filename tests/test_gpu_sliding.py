@@ -141,6 +141,8 @@ def test_one_visible_key_has_no_score_gradient():
     q, k, v = (make(i, 1, 200, 2, 64).requires_grad_() for i in (1, 2, 3))
     o = sliding_window_attention(q, k, v, 1)
     dq, dk, dv = torch.autograd.grad(o, [q, k, v], make(4, 1, 200, 2, 64))
+    wide = sliding_window_attention(q, k, v, 2 ** 40)  # any whole number is a window
+    assert torch.equal(wide, sliding_window_attention(q, k, v, 200))
     assert torch.equal(o, v) and not dq.any() and not dk.any() and torch.equal(dv, make(4, 1, 200, 2, 64))
 
 

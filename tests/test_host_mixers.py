@@ -131,7 +131,7 @@ def test_layer_norm_codes(rows, n, dx, dr, dw, st):
 
 @pytest.mark.parametrize("B,T,D,dx,dg,st", [
     (0, 1, 1, 0, 0, VAL), (1, 0, 1, 0, 0, VAL), (1, 1, 0, 0, 0, VAL), (1, 1, 1, 0, 1, NOT),
-    (1, 1, 1, 5, 5, NOT), (1 << 20, 1 << 20, 64, 0, 0, NOT), (1, 8, 8, 0, 2, VAL)])
+    (1, 1, 1, 5, 5, NOT), (1, 2 ** 30 + 1, 1, 2, 2, NOT), (1 << 20, 1 << 20, 64, 0, 0, NOT), (1, 8, 8, 0, 2, VAL)])
 def test_recurrence_codes(B, T, D, dx, dg, st):
     assert code("hattn_gated_recurrence_fwd", *([None] * 7), B, T, D, dx, dg, None, 0, None) == st
     assert code("hattn_gated_recurrence_bwd", *([None] * 9), B, T, D, dx, dg, None, 0, None) == st
