@@ -44,7 +44,9 @@ __device__ __forceinline__ floatx16 zero16() {
 }
 
 // max(a, b, c) as one instruction: fmaxf would first quiet each operand by one of its own.
-// A NaN operand is ignored.
+// A NaN operand is ignored.  The compiler places no wait between a matrix product and inline
+// assembly that reads it, so `a` comes from an ordinary instruction that has read b's and c's
+// product before.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -124,25 +126,10 @@ struct TileLoad {
   }
 };
 
-// Waits until at most N of this wave's loads are in flight.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N < 16);
-  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
-}
-
 // Waits for this wave's asynchronous loads, then for the other waves.
 __device__ __forceinline__ void tile_barrier() {
-  wait_loads<0>();
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
-}
-
-// A barrier that leaves asynchronous loads in flight (__syncthreads waits for them): this
-// wave's reads of LDS are done before it, and none moves across it.
-__device__ __forceinline__ void phase_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // The B operand rows of one matrix, kept in registers: row `src` of this lane (ln),

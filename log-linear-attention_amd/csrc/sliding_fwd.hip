@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 3) void sliding_fwd_kernel(Slid
   const int tiles = keys.tiles();
   const TileLoad<DP, BN, 4> tile(p.D);
 
-  float m = -1e30f, l = 0.f;
+  float m = -3e38f, l = 0.f;  // below every score; not -inf, whose difference is NaN
   const auto part = [&](auto MASK, int j, int kt, int kind, const __bf16* K, const __bf16* V)
                         __attribute__((always_inline)) {
     floatx16 s = zero16();

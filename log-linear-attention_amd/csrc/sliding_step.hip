@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256, 2) void sliding_step_kernel(SlidingStepArgs p)
           (__attribute__((address_space(3))) void*)(V + wave * 32 * DP + i * 512), 16, 0, 0);
     }
   };
-  float m = -1e30f, l = 0.f;
+  float m = -3e38f, l = 0.f;  // below every score; not -inf, whose difference is NaN
   floatx4 acc[DP / 16];
 #pragma unroll
   for (int dt = 0; dt < DP / 16; ++dt) acc[dt] = zero4();

@@ -137,6 +137,20 @@ def test_peaked_scores():
     close("o", o, want["o"], tol["o"])
 
 
+def test_scores_far_below_zero():
+    """The largest score of a row is far below anything that a softmax usually meets."""
+    B, T, H, D = 1, 200, 1, 64
+    q = torch.full((B, T, H, D), 2.0 ** 60, device=DEV, dtype=BF)
+    k = torch.full((B, T, H, D), -2.0 ** 58, device=DEV, dtype=BF)
+    v = make(3, B, T, H, D)
+    want, tol = oracle(torch.zeros_like(q), k, v, 90, 4)  # equal scores: the keys' mean
+    close("o", sliding_window_attention(q, k, v, 90, 4), want["o"], tol["o"])
+    state = SlidingState.empty(B, H, D, 90, 4, device=DEV)
+    for t in range(120):
+        o, _ = sliding_window_step(state, q[:, t], k[:, t], v[:, t])
+    close("step", o, want["o"][:, 119], tol["o"][:, 119])
+
+
 def test_one_visible_key_has_no_score_gradient():
     q, k, v = (make(i, 1, 200, 2, 64).requires_grad_() for i in (1, 2, 3))
     o = sliding_window_attention(q, k, v, 1)
