@@ -694,8 +694,10 @@ int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, c
  * ignored.  Where x has 16 bits and D is even, x, g, o and the gradients are aligned to two of
  * their elements.
  *
- * Workgroups wait, with a bounded poll, for the states of earlier segments; a wait that
- * gives up (two calls that overlap on one workspace) gives NaN, not plausible numbers.
+ * Workgroups take the segments in order from a counter in the workspace and wait, with a
+ * bounded poll, for the states of earlier ones; a wait that gives up gives NaN.  Calls that may
+ * overlap (on two streams, in two graphs) need a workspace each: on one they stay in bounds,
+ * but the results are undefined.
  */
 int hattn_gated_recurrence_segments(int T, int D, int dtype_x);
 size_t hattn_gated_recurrence_workspace(int B, int T, int D, int dtype_x);

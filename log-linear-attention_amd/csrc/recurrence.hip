@@ -21,9 +21,11 @@
 //
 // A word is 64 bits wide and is written and read by one atomic access of device
 // scope, so it is its own flag: kEmpty (a NaN pattern that publish() never writes)
-// until it holds a map.  A workgroup waits only for workgroups that come before it
-// in the order of dispatch; the wait is bounded, and one that gives up makes its
-// outputs NaN.
+// until it holds a map.  Segments are handed out by one counter in the order of the walk, so
+// a workgroup waits only for workgroups that already run, wherever and whenever the card
+// starts them and whatever else runs beside (each XCD starts its own share of a grid in order,
+// which does not order the whole).  The wait is bounded all the same, and one that gives up
+// makes its outputs NaN.
 #include "common.h"
 #include "recurrence.h"
 
@@ -99,24 +101,41 @@ __device__ __forceinline__ float look_back(const unsigned long long* w, long ste
   return h;
 }
 
-__global__ void fill_empty_kernel(unsigned long long* w, long n) {
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-       i += (long)gridDim.x * blockDim.x)
-    w[i] = kEmpty;
+// The counter of the segments lies in the first word of the last segment of the walk, which
+// no other segment reads.
+__device__ __host__ __forceinline__ long counter_word(const RecurrenceArgs& p, bool backward) {
+  return backward ? 0 : (long)(p.nseg - 1) * p.B * p.strips * 64 * p.vec;
 }
 
-// blockIdx.x = segment * units + unit, unit = batch * strips + strip of 64 lanes:
-// every unit's first segment is dispatched first.
+__global__ void fill_empty_kernel(unsigned long long* w, long n, long counter) {
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (long)gridDim.x * blockDim.x)
+    w[i] = i == counter ? 0 : kEmpty;
+}
+
+// The workgroup's item = step of the walk * units + unit, unit = batch * strips + strip of 64
+// lanes: every unit's first segment comes first.  Items past the last are only handed out where
+// another call resets the counter meanwhile: such a workgroup does nothing.
+__device__ __forceinline__ unsigned take_item(const RecurrenceArgs& p, bool backward) {
+  if (p.nseg == 1) return blockIdx.x;
+  __shared__ unsigned ticket;
+  if (threadIdx.x == 0)
+    ticket = __hip_atomic_fetch_add(
+        (unsigned*)((unsigned long long*)p.ws + counter_word(p, backward)), 1u, __ATOMIC_RELAXED,
+        __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(ticket);
+}
 struct Place {
   int b, d, seg, len;
   long unit;
   bool live;  // all of a lane's channels are there or none
 };
 template <int VEC>
-__device__ __forceinline__ Place place(const RecurrenceArgs& p, bool backward) {
+__device__ __forceinline__ Place place(const RecurrenceArgs& p, unsigned item, bool backward) {
   Place at;
   const int units = p.B * p.strips;
-  const int u = blockIdx.x % units, s = blockIdx.x / units;
+  const int u = item % units, s = item / units;
   at.seg = backward ? p.nseg - 1 - s : s;
   at.unit = u;
   at.b = u / p.strips;
@@ -156,7 +175,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(Recurren
   constexpr int TOK = kTok<VEC>;
   __shared__ Map maps[kWaves][VEC][64];
   __shared__ float enter[VEC][64];
-  const Place at = place<VEC>(p, false);
+  const unsigned item = take_item(p, false);
+  if (item >= gridDim.x) return;
+  const Place at = place<VEC>(p, item, false);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = (at.seg * kWaves + wave) * TOK;
   const int d = at.live ? at.d : 0;
@@ -236,7 +257,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(Recurren
   constexpr int TOK = kTok<VEC>;
   __shared__ Map fwd[kWaves][VEC][64], bwd[kWaves][VEC][64];
   __shared__ float enter[VEC][64];
-  const Place at = place<VEC>(p, true);
+  const unsigned item = take_item(p, true);
+  if (item >= gridDim.x) return;
+  const Place at = place<VEC>(p, item, true);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = (at.seg * kWaves + wave) * TOK;
   const int d = at.live ? at.d : 0;
@@ -350,7 +373,7 @@ static hipError_t launch_scan(int what, const RecurrenceArgs& p, hipStream_t str
     const long n = units * 64 * VEC * p.nseg;
     const long want = (n + 1023) / 1024;
     hipLaunchKernelGGL(fill_empty_kernel, dim3((unsigned)(want < 1024 ? want : 1024)), dim3(256), 0,
-                       stream, (unsigned long long*)p.ws, n);
+                       stream, (unsigned long long*)p.ws, n, counter_word(p, what == 1));
   }
   const dim3 grid((unsigned)(units * p.nseg)), block(64 * kWaves);
   if (what == 0)
