@@ -683,7 +683,8 @@ int hattn_layer_norm_bwd(const void* s, const void* weight, const float* mean, c
                          void* ws, size_t ws_bytes, void* stream);
 
 /*
- * Gated linear recurrence, per channel: h_t = exp(g_t) h_{t-1} + x_t, o_t = h_t.
+ * Gated linear recurrence, per channel: h_t = exp(g_t) h_{t-1} + x_t, o_t = h_t.  States that
+ * are not finite stay so.  The product of exp(g) over 256 tokens stays in fp32's range.
  * x, o [B, T, D] in dtype_x; g [B, T, D] in dtype_g (dtype_x or FP32); h0, ht [B, D] fp32
  * state before and after, each may be NULL (h0: zero); lengths [B] int32 or NULL: row b
  * has lengths[b] tokens (clamped to [0, T]), its later outputs are zero, its later inputs

@@ -14,14 +14,16 @@
 //
 // Inside the workgroup the waves' maps meet in LDS; between the segments of a channel the
 // workgroup publishes its map in a word {A, X} and then walks back over the words before it
-// until one has A = 0.  A segment whose state is known replaces its word by {0, h}, so the
-// walk is short, and the data is read once and written once: bound by the bytes (forward
+// until one holds a state.  A segment whose state is known replaces its word by {kState, h}, so
+// the walk is short, and the data is read once and written once: bound by the bytes (forward
 // 4.3 TB/s and backward 5.0 at the shape above in bf16, forward 4.9 at B 1, T 131072, D 1024
 // in fp32).
 //
 // A word is 64 bits wide and is written and read by one atomic access of device
 // scope, so it is its own flag: kEmpty (a NaN pattern that publish() never writes)
-// until it holds a map.  Segments are handed out by one counter in the order of the walk, so
+// until it holds a map.  No map drops what comes before it: a state that is not finite passes
+// it as it passes the tokens, also where the product of decays that are not zero falls below
+// fp32's range, which is kept as its smallest number (compose() below).  Segments are handed out by one counter in the order of the walk, so
 // a workgroup waits only for workgroups that already run, wherever and whenever the card
 // starts them and whatever else runs beside (each XCD starts its own share of a grid in order,
 // which does not order the whole).  The wait is bounded all the same, and one that gives up
@@ -35,6 +37,7 @@ constexpr int kWaves = 8;                // waves a workgroup
 template <int VEC>
 constexpr int kTok = 32 / VEC;           // tokens a wave
 constexpr unsigned long long kEmpty = ~0ull;
+constexpr unsigned kState = 0x7fc00001u;  // in place of A: the word holds a state (a NaN pattern too)
 constexpr int kSpins = 1 << 20;          // rounds of a wait, about a second
 
 struct Map {
@@ -45,24 +48,48 @@ __device__ __forceinline__ float no_payload(float x) {
   return x != x ? __builtin_bit_cast(float, 0x7fc00000u) : x;
 }
 
-__device__ __forceinline__ void publish(unsigned long long* w, float A, float X) {
-  const unsigned lo = __builtin_bit_cast(unsigned, no_payload(A));
+__device__ __forceinline__ void put_word(unsigned long long* w, unsigned lo, float X) {
   const unsigned hi = __builtin_bit_cast(unsigned, no_payload(X));
   __hip_atomic_store(w, (unsigned long long)hi << 32 | lo, __ATOMIC_RELAXED,
                      __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish(unsigned long long* w, Map m) {
+  put_word(w, __builtin_bit_cast(unsigned, no_payload(m.A)), m.X);
+}
+__device__ __forceinline__ void publish_state(unsigned long long* w, float h) {
+  put_word(w, kState, h);
 }
 
 __device__ __forceinline__ unsigned long long word(const unsigned long long* w) {
   return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ float apply(Map m, float h) { return __builtin_fmaf(m.A, h, m.X); }
 __device__ __forceinline__ float apply(unsigned long long w, float h) {
-  const float A = __builtin_bit_cast(float, (unsigned)w);
   const float X = __builtin_bit_cast(float, (unsigned)(w >> 32));
-  return A == 0.f ? X : A * h + X;
+  return (unsigned)w == kState ? X : apply(Map{__builtin_bit_cast(float, (unsigned)w), X}, h);
+}
+
+// A product of decays, `zero` where one of them is zero.  One that only underflowed is kept as
+// the smallest number, so that infinity stays infinity; it adds at most 5e-7 to a state whose
+// predecessor is 3e38.
+__device__ __forceinline__ float no_underflow(float A, bool zero) {
+  return A == 0.f && !zero ? __builtin_bit_cast(float, 1u) : A;
+}
+template <int TOK, int VEC>
+__device__ __forceinline__ float no_underflow(float A, const float (&a)[TOK][VEC], int e) {
+  if (!__any(A == 0.f)) return A;
+  bool zero = false;
+#pragma unroll
+  for (int i = 0; i < TOK; ++i) zero |= a[i][e] == 0.f;
+  return no_underflow(A, zero);
+}
+// n after m
+__device__ __forceinline__ Map compose(Map n, Map m) {
+  return Map{no_underflow(n.A * m.A, n.A == 0.f || m.A == 0.f), apply(n, m.X)};
 }
 
 // The state that enters this segment from the words of the `before` segments before
-// it (w[0], w[step], ..): back to the nearest one whose words all have A = 0, or to
+// it (w[0], w[step], ..): back to the nearest one whose words all hold a state, or to
 // the first segment and `base`, then their maps forward from there.  The state is
 // built in the order of the tokens wherever the walk starts, so its bits do not
 // depend on which words were already replaced.
@@ -82,7 +109,7 @@ __device__ __forceinline__ float look_back(const unsigned long long* w, long ste
     for (int i = 0; i < N; ++i)
       if (used == i && !found && n + i < before && !__any(got[i] == kEmpty)) {
         ++used;
-        found = __all((unsigned)got[i] << 1 == 0);
+        found = __all(!live || (unsigned)got[i] == kState);
       }
     n += used;
     if (found) break;
@@ -206,7 +233,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(Recurren
       X = a[i][e] * X + v[i][e];
       A *= a[i][e];
     }
-    maps[wave][e][lane] = Map{A, X};
+    maps[wave][e][lane] = Map{no_underflow(A, a, e), X};
   }
   __syncthreads();
   // the first waves join the maps, one for each of a lane's channels
@@ -214,20 +241,16 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(Recurren
     const int e = wave;
     Map m = maps[0][e][lane];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) {
-      const Map n = maps[k][e][lane];
-      m = Map{n.A * m.A, n.A * m.X + n.X};
-    }
+    for (int k = 1; k < kWaves; ++k) m = compose(maps[k][e][lane], m);
     const float h0 = p.h0 && at.live ? p.h0[(long)at.b * p.D + d + e] : 0.f;
     const long stride = (long)p.B * p.strips * 64 * VEC;
     unsigned long long* w =
         (unsigned long long*)p.ws + at.seg * stride + (at.unit * VEC + e) * 64 + lane;
     const bool last = at.seg == p.nseg - 1;
-    if (at.live && !last && at.seg > 0) publish(w, m.A, m.X);
+    if (at.live && !last && at.seg > 0) publish(w, m);
     const float h = look_back(w - stride, -stride, at.seg, h0, at.live);
-    // as apply(): A = 0 ends a walk, so nothing before such a segment reaches past it
-    const float out = m.A == 0.f ? m.X : m.A * h + m.X;
-    if (at.live && !last) publish(w, 0.f, out);
+    const float out = apply(m, h);
+    if (at.live && !last) publish_state(w, out);
     if (at.live && last && p.ht) p.ht[(long)at.b * p.D + d + e] = out;
     if (at.live && p.carry) p.carry[((long)at.b * p.nseg + at.seg) * p.D + d + e] = h;
     enter[e][lane] = h;
@@ -237,7 +260,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_fwd_kernel(Recurren
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     h[e] = enter[e][lane];
-    for (int k = 0; k < wave; ++k) h[e] = maps[k][e][lane].A * h[e] + maps[k][e][lane].X;
+    for (int k = 0; k < wave; ++k) h[e] = apply(maps[k][e][lane], h[e]);
   }
   TX* o = (TX*)p.o + base;
 #pragma unroll
@@ -291,6 +314,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(Recurren
     }
 #pragma unroll
     for (int i = TOK - 1; i >= 0; --i) E = a[i][e] * (q[i][e] + E);
+    A = no_underflow(A, a, e);
     fwd[wave][e][lane] = Map{A, X};
     bwd[wave][e][lane] = Map{A, E};
   }
@@ -299,19 +323,16 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(Recurren
     const int e = wave;
     Map m = bwd[kWaves - 1][e][lane];
 #pragma unroll
-    for (int k = kWaves - 2; k >= 0; --k) {
-      const Map n = bwd[k][e][lane];
-      m = Map{n.A * m.A, n.A * m.X + n.X};
-    }
+    for (int k = kWaves - 2; k >= 0; --k) m = compose(bwd[k][e][lane], m);
     const float end = p.ght && at.live ? p.ght[(long)at.b * p.D + d + e] : 0.f;
     const long stride = (long)p.B * p.strips * 64 * VEC;
     unsigned long long* w =
         (unsigned long long*)p.ws + at.seg * stride + (at.unit * VEC + e) * 64 + lane;
     const int after = p.nseg - 1 - at.seg;
-    if (at.live && after > 0 && at.seg > 0) publish(w, m.A, m.X);
+    if (at.live && after > 0 && at.seg > 0) publish(w, m);
     const float in = look_back(w + stride, stride, after, end, at.live);
-    const float out = m.A == 0.f ? m.X : m.A * in + m.X;
-    if (at.live && at.seg > 0) publish(w, 0.f, out);
+    const float out = apply(m, in);
+    if (at.live && at.seg > 0) publish_state(w, out);
     if (at.live && at.seg == 0 && p.dh0) p.dh0[(long)at.b * p.D + d + e] = out;
     enter[e][lane] = in;
   }
@@ -319,7 +340,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(Recurren
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     float h = p.carry[((long)at.b * p.nseg + at.seg) * p.D + d + e];
-    for (int k = 0; k < wave; ++k) h = fwd[k][e][lane].A * h + fwd[k][e][lane].X;
+    for (int k = 0; k < wave; ++k) h = apply(fwd[k][e][lane], h);
 #pragma unroll
     for (int i = 0; i < TOK; ++i) {
       const float was = h;
@@ -332,7 +353,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void recurrence_bwd_kernel(Recurren
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
     s[e] = enter[e][lane];
-    for (int k = kWaves - 1; k > wave; --k) s[e] = bwd[k][e][lane].A * s[e] + bwd[k][e][lane].X;
+    for (int k = kWaves - 1; k > wave; --k) s[e] = apply(bwd[k][e][lane], s[e]);
   }
   TX* dx = (TX*)p.dx + base;
   TG* dg = (TG*)p.dg + base;

@@ -104,7 +104,8 @@ def gated_linear_recurrence(x: torch.Tensor, g: torch.Tensor,
     """``o_t = h_t = exp(g_t) h_{t-1} + x_t`` for each channel.
 
     x [B, T, D] (bf16, fp16 or fp32), g [B, T, D] log-decays in x's dtype or fp32 (-inf
-    resets the channel), initial_state [B, D] (zero where None), lengths [B] (int32 or
+    resets a channel whose state is finite; the product of exp(g) over 256 tokens has to
+    stay in fp32's range, as that of decays does), initial_state [B, D] (zero where None), lengths [B] (int32 or
     int64, on the device) the tokens of each row of a padded batch: outputs and gradients
     past them are zero, inputs past them are not used.  Returns o in x's dtype, or with
     ``output_final_state`` ``(o, ht)``, ht [B, D] fp32 the state after each row's last
