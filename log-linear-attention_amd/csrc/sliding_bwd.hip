@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void sliding_bwd_q_kernel(Sl
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = zero16();
   if (t0 >= len) {
-    if (t < p.T) store_t<E, DP>(dq, acc, 0.f, p.D);
+    if (t < p.T) store_t<E, DP>(dq, acc, 0.f, false, p.D);
     return;
   }
   const __bf16* k = (const __bf16*)p.k + b * p.kb + g * p.kh;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void sliding_bwd_q_kernel(Sl
   for (; j < tiles && !(j >= lo && j + 2 <= hi); j += 2) pairs(Bool<true>(), Bool<false>());
   for (; j + 2 <= hi; j += 2) pairs(Bool<false>(), Bool<false>());
   for (; j < tiles; j += 2) pairs(Bool<true>(), Bool<false>());
-  if (t < p.T) store_t<E, DP>(dq, acc, t < len ? p.scale : 0.f, p.D);
+  if (t < p.T) store_t<E, DP>(dq, acc, p.scale, t < len, p.D);
 }
 
 // dK and dV.  SINKS false: 128 keys a workgroup, 32 a wave, over the queries whose window
@@ -264,6 +264,7 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
     if (j + 1 < tiles) step(j + 1, Q1, O1, st1, Q0, O0, st0);
   }
 
+  const bool live = key < len;  // the others' sums are zero, or 0 times what is not finite
   // row (slot, b, g, key) of the partial sums: D of dK, D of dV
   float* part = p.part + ((((long)slot * p.B + b) * p.G + g) * p.S + key) * 2 * p.D;
   const auto put = [&](const floatx16(&acc)[DP / 32], float* dst) __attribute__((always_inline)) {
@@ -273,8 +274,9 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * dt + 8 * i + 4 * hf;
         if (d < p.D)
-          *(floatx4*)(dst + d) = floatx4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2],
-                                         acc[dt][4 * i + 3]};
+          *(floatx4*)(dst + d) = live ? floatx4{acc[dt][4 * i], acc[dt][4 * i + 1],
+                                                acc[dt][4 * i + 2], acc[dt][4 * i + 3]}
+                                      : floatx4{};
       }
   };
   if constexpr (SINKS) {
@@ -308,8 +310,8 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
       return;
     }
     const long row = (((long)b * p.T + key) * p.G + g) * p.D;
-    store_t<E, DP>((__bf16*)p.dk + row, dk, p.scale, p.D);
-    store_t<E, DP>((__bf16*)p.dv + row, dv, 1.f, p.D);
+    store_t<E, DP>((__bf16*)p.dk + row, dk, p.scale, live, p.D);
+    store_t<E, DP>((__bf16*)p.dv + row, dv, 1.f, live, p.D);
   }
 }
 

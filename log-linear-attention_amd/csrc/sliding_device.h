@@ -145,10 +145,11 @@ __device__ __forceinline__ void load_frags(const __bf16* src, int D, bf16x8 (&f)
 }
 
 // Stores a transposed result: X[d][row = ln], acc tile dt has d = 32 dt + 8 (i >> 2) +
-// 4 hf + (i & 3); dst: this lane's row.
+// 4 hf + (i & 3); dst: this lane's row.  Rows that are not live are zero, whatever acc holds (a
+// padded row's lane repeats the last live one, which need not be finite).
 template <typename E, int DP>
 __device__ __forceinline__ void store_t(__bf16* dst, const floatx16 (&acc)[DP / 32], float scale,
-                                        int D) {
+                                        bool live, int D) {
   const int hf = threadIdx.x >> 5 & 1;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -157,7 +158,7 @@ __device__ __forceinline__ void store_t(__bf16* dst, const floatx16 (&acc)[DP / 
       const int d = 32 * dt + 8 * i + 4 * hf;
       bf16x4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = to16<E>(acc[dt][4 * i + j] * scale);
+      for (int j = 0; j < 4; ++j) x[j] = to16<E>(live ? acc[dt][4 * i + j] * scale : 0.f);
       if (d < D) *(bf16x4*)(dst + d) = x;
     }
 }

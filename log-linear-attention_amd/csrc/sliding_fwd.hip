@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 3) void sliding_fwd_kernel(Slid
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = zero16();
   if (t0 >= len) {
-    if (t < p.T) store_t<E, DP>(out, acc, 0.f, p.D);
+    if (t < p.T) store_t<E, DP>(out, acc, 0.f, false, p.D);
     return;
   }
   const __bf16* k = (const __bf16*)p.k + b * p.kb + g * p.kh;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 3) void sliding_fwd_kernel(Slid
   for (; j + 2 <= hi; j += 2) pairs(Bool<false>());
   for (; j < tiles; j += 2) pairs(Bool<true>());
   l += __shfl_xor(l, 32, 64);
-  if (t < p.T) store_t<E, DP>(out, acc, t < len ? 1.f / l : 0.f, p.D);
+  if (t < p.T) store_t<E, DP>(out, acc, 1.f / l, t < len, p.D);
   if (lse && t < len && hf == 0) *lse = m + log2f(l);
 }
 
