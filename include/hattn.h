@@ -654,7 +654,10 @@ int hattn_gated_rmsnorm_bwd(const void* y, const void* z, long long ldz, const v
 /*
  * Mixers and norm of a hybrid stack, next to the log-linear scans.  No counterpart in
  * the reference.  Invalid sizes are HATTN_ERR_VALUE, sizes and types outside what is
- * built HATTN_ERR_NOT_IMPLEMENTED.
+ * built HATTN_ERR_NOT_IMPLEMENTED, and so are sizes whose launch would have 2^32 threads or
+ * more: for the recurrence 2^23 workgroups (of a row, a segment and 64 channels, or 128 where
+ * they go two to a lane) or 2^32 channels a step, for the attention 2^24 (of a row, a head and
+ * 128 queries; while decoding of a row and key head, and its parts) or a cache of 2^35 values.
  */
 
 /*

@@ -3,6 +3,7 @@
 // All checks are made here, on the host; the kernels assume what they establish.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 
@@ -20,6 +21,13 @@ const float kLog2e = 1.4426950408889634f;
 
 // The attention kernels address the rows of one tile by 32-bit offsets.
 const long long kMaxTokenStride = 1LL << 24;
+
+// Slots of a cache: the step rounds its runs of slots up, by 32 in each of 256.
+const long long kMaxSlots = INT_MAX - (1 << 14);
+
+// Whether n work items, `per` a workgroup (or workgroups in groups of `per`), make a launch: it
+// holds at most 2^32 - 1 threads.
+bool fits(double n, int per, int threads) { return std::ceil(n / per) * threads < 4294967296.0; }
 
 int check_dtype(int code, const char* what) {
   if (code < HATTN_BF16 || code > HATTN_FP32)
@@ -49,21 +57,26 @@ RecurrenceArgs recurrence_shape(int B, int T, int D, int dtype_x) {
   RecurrenceArgs p{};
   p.B = B; p.T = T; p.D = D;
   p.vec = dtype_x != HATTN_FP32 && D % 2 == 0 ? 2 : 1;
-  p.strips = (D + 64 * p.vec - 1) / (64 * p.vec);
+  p.strips = (D - 1) / (64 * p.vec) + 1;
   const int tokens = hattn_recurrence_segment(p.vec);
   p.nseg = (T - 1) / tokens + 1;
   return p;
 }
 
-int recurrence_checks(int B, int T, int D, int dtype_x, int dtype_g) {
+int recurrence_types(int B, int T, int D, int dtype_x, int dtype_g) {
   if (B <= 0 || T <= 0 || D <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (int st = check_dtype(dtype_x, "x")) return st;
   if (dtype_g != dtype_x && dtype_g != HATTN_FP32)
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "g of dtype code %d with x of %d", dtype_g, dtype_x);
+  return HATTN_OK;
+}
+
+int recurrence_checks(int B, int T, int D, int dtype_x, int dtype_g) {
+  if (int st = recurrence_types(B, T, D, dtype_x, dtype_g)) return st;
   if (T > (1 << 30)) return fail(HATTN_ERR_NOT_IMPLEMENTED, "T=%d above 2^30", T);
   const RecurrenceArgs p = recurrence_shape(B, T, D, dtype_x);
-  if ((long long)p.B * p.strips * p.nseg >= (1LL << 31))
-    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d D=%d: 2^31 segments", B, T, D);
+  if (!fits((double)p.B * p.strips * p.nseg, 1, 512))
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d D=%d: 2^23 workgroups or more", B, T, D);
   return HATTN_OK;
 }
 
@@ -116,15 +129,27 @@ int stride_checks(const long long* st, int n) {
   return HATTN_OK;
 }
 
+// Workgroups of the forward (and of dQ's kernel), and with `train` of the backward's others.
+int sliding_grids(int B, int T, int H, int G, int D, int window, int sinks, bool train) {
+  const long long rows = T / 128 + (T % 128 != 0);
+  const int W = std::min(window, T), S = std::min(sinks, T);
+  const long long far = S > 0 ? (T - W) / kSinkChunk + ((T - W) % kSinkChunk != 0) : 0;
+  bool ok = T <= INT_MAX / 2 && fits((double)B * H * rows, 8, 8 * 256);
+  if (train && far > 0)
+    ok = ok && fits((double)B * H * far * ((S + 31) / 32), 8, 8 * 256) &&
+         fits((double)B * G * S * 2 * D, 256, 256);
+  return ok ? HATTN_OK
+            : fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: 2^24 workgroups or more", B, T, H);
+}
+
 int sliding_fill(SlidingArgs& p, const void* q, const void* k, const void* v, const int* lengths,
                  const long long* strides, int B, int T, int H, int G, int D, int window, int sinks,
-                 float scale, int dtype) {
+                 float scale, int dtype, bool train) {
   if (T <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (int st = sliding_checks(B, H, G, D, window, sinks, scale, dtype)) return st;
+  if (int st = sliding_grids(B, T, H, G, D, window, sinks, train)) return st;
   if (!q || !k || !v || !strides) return fail(HATTN_ERR_VALUE, "null tensor pointer");
   if (int st = stride_checks(strides, 9)) return st;
-  if ((long long)B * H * ((T + 127) / 128) >= (1LL << 31) - 8 || T > INT_MAX / 2)
-    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: too many blocks", B, T, H);
   p = SlidingArgs{};
   p.q = q; p.k = k; p.v = v; p.lengths = lengths;
   p.qb = strides[0]; p.qt = strides[1]; p.qh = strides[2];
@@ -225,7 +250,9 @@ int hattn_gated_recurrence_bwd(const void* x, const void* g, const float* carry,
 
 int hattn_gated_recurrence_step(float* state, const void* x, const void* g, void* o, int B, int D,
                                 int dtype_x, int dtype_g, void* stream) {
-  if (int st = recurrence_checks(B, 1, D, dtype_x, dtype_g)) return st;
+  if (int st = recurrence_types(B, 1, D, dtype_x, dtype_g)) return st;
+  if (!fits((double)B * D, 256, 256))
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d D=%d: 2^32 channels or more", B, D);
   if (!state || !x || !g || !o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
   RecurrenceArgs p{};
   p.x = x; p.g = g; p.o = o; p.ht = state;
@@ -238,7 +265,9 @@ int hattn_sliding_fwd(const void* q, const void* k, const void* v, const int* le
                       const long long* strides, void* o, float* lse, int B, int T, int H, int G,
                       int D, int window, int sinks, float scale, int dtype, void* stream) {
   SlidingArgs p;
-  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype))
+  // with lse a backward follows: what it refuses is refused here
+  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype,
+                            lse != nullptr))
     return st;
   if (!o) return fail(HATTN_ERR_VALUE, "null tensor pointer");
   if (!aligned({q, k, v, o}, 16)) return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
@@ -251,6 +280,7 @@ int hattn_sliding_fwd(const void* q, const void* k, const void* v, const int* le
 size_t hattn_sliding_bwd_workspace(int B, int T, int H, int G, int D, int window, int sinks) {
   if (B <= 0 || T <= 0 || D <= 0 || window < 1 || sinks < 0 || G <= 0 || H < G) return 0;
   const int S = std::min(sinks, T);
+  if (S > kMaxSinks || sliding_grids(B, T, H, G, D, window, sinks, true)) return 0;
   return sliding_bwd_delta(B, T, H) + (size_t)sliding_sink_slots(T, H, G, std::min(window, T), S) *
                                           B * G * S * 2 * D * sizeof(float);
 }
@@ -260,7 +290,8 @@ int hattn_sliding_bwd(const void* q, const void* k, const void* v, const int* le
                       void* dq, void* dk, void* dv, int B, int T, int H, int G, int D, int window,
                       int sinks, float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
   SlidingArgs p;
-  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype))
+  if (int st = sliding_fill(p, q, k, v, lengths, strides, B, T, H, G, D, window, sinks, scale, dtype,
+                            true))
     return st;
   if (!o || !lse || !dout || !dq || !dk || !dv) return fail(HATTN_ERR_VALUE, "null tensor pointer");
   if (!aligned({q, k, v, o, dout, dq, dk, dv, ws}, 16))
@@ -283,14 +314,15 @@ int hattn_sliding_cache_fill(const void* k, const void* v, const int* lengths,
                              void* stream) {
   if (T <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (int st = sliding_checks(B, G, G, D, window, sinks, 1.f, dtype)) return st;
+  if ((long long)window + sinks > INT_MAX ||
+      !fits((double)B * G * ((double)sinks + window) * (D / 8), 256, 256))
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d G=%d window=%d: a cache of 2^32 pieces or more", B, G,
+                window);
   if (!k || !v || !strides || !k_cache || !v_cache || !counts)
     return fail(HATTN_ERR_VALUE, "null tensor pointer");
   if (int st = stride_checks(strides, 6)) return st;
   if (!aligned({k, v, k_cache, v_cache}, 16))
     return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
-  if ((long long)window + sinks > INT_MAX ||
-      (long long)B * G * ((long long)sinks + window) * (D / 8) / 256 >= INT_MAX)
-    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d G=%d window=%d: cache too large", B, G, window);
   SlidingStepArgs p{};
   p.k = k; p.v = v; p.kc = k_cache; p.vc = v_cache; p.counts = counts;
   p.B = B; p.G = G; p.D = D; p.W = window; p.S = sinks;
@@ -302,7 +334,7 @@ int hattn_sliding_cache_fill(const void* k, const void* v, const int* lengths,
 
 size_t hattn_sliding_step_workspace(int B, int H, int G, int D, int window, int sinks) {
   if (B <= 0 || G <= 0 || H < G || D <= 0 || window < 1 || sinks < 0 ||
-      (long long)window + sinks > INT_MAX)
+      (long long)window + sinks > kMaxSlots)
     return 0;
   return (size_t)B * H * step_splits(B, H, G, window + sinks) * (D + 2) * sizeof(float);
 }
@@ -311,22 +343,23 @@ int hattn_sliding_step(const void* q, const void* k, const void* v, void* k_cach
                        int* counts, void* o, int B, int H, int G, int D, int window, int sinks,
                        float scale, int dtype, void* ws, size_t ws_bytes, void* stream) {
   if (int st = sliding_checks(B, H, G, D, window, sinks, scale, dtype)) return st;
+  if ((long long)window + sinks > kMaxSlots)
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "window=%d too large", window);
+  const int splits = step_splits(B, H, G, window + sinks), rblocks = (H / G + 15) / 16;
+  if (!fits((double)B * G * rblocks * splits, 1, 256) || !fits((double)B * H, 1, 128))
+    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d H=%d: too many rows", B, H);
   if (!q || !k || !v || !k_cache || !v_cache || !counts || !o)
     return fail(HATTN_ERR_VALUE, "null tensor pointer");
   if (!aligned({q, k, v, k_cache, v_cache, ws}, 16))
     return fail(HATTN_ERR_VALUE, "tensor not aligned to 16 bytes");
-  if ((long long)window + sinks > INT_MAX - 256)
-    return fail(HATTN_ERR_NOT_IMPLEMENTED, "window=%d too large", window);
   const size_t need = hattn_sliding_step_workspace(B, H, G, D, window, sinks);
   if (!ws || ws_bytes < need)
     return fail(HATTN_ERR_VALUE, "workspace of %zu bytes, %zu needed", ws_bytes, need);
   SlidingStepArgs p{};
   p.q = q; p.k = k; p.v = v; p.kc = k_cache; p.vc = v_cache; p.counts = counts; p.o = o;
   p.B = B; p.H = H; p.G = G; p.D = D; p.W = window; p.S = sinks;
-  p.splits = step_splits(B, H, G, window + sinks);
-  p.rblocks = (H / G + 15) / 16;
-  if ((long long)B * G * p.rblocks * p.splits > INT_MAX || (long long)B * H > INT_MAX)
-    return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d H=%d: too many rows", B, H);
+  p.splits = splits;
+  p.rblocks = rblocks;
   p.scale2 = scale * kLog2e;
   p.part = (float*)ws;
   p.stat = p.part + (size_t)B * H * p.splits * D;
