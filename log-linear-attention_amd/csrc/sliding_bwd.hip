@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void sliding_bwd_q_kernel(Sl
           const TileMask seen(keys, j, t, p.W, p.S);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            s[i] = seen(32 * kt + 8 * (i >> 2) + (i & 3)) & !alone ? s[i] : 0.f;
+            s[i] = (seen(32 * kt + 8 * (i >> 2) + (i & 3)) & !alone) ? s[i] : 0.f;
         }
       }
       if constexpr (DELTA.value) {
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256, DP == 64 && !SINKS ? 2 : 1) void sliding_bwd_k
           const int place = 8 * (i >> 2) + (i & 3);
           const bool seen = (place >= low) & (place <= up);
           s[i] = seen ? s[i] : 0.f;
-          dp[i] = seen & (place > one) ? dp[i] : 0.f;
+          dp[i] = (seen & (place > one)) ? dp[i] : 0.f;
         }
       }
 #pragma unroll
