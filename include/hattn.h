@@ -731,9 +731,16 @@ int hattn_gated_recurrence_step(float* state, const void* x, const void* g, void
  * each a multiple of 8 (the last dimension is contiguous); o [B, T, H, D] contiguous;
  * lse [B, H, T] fp32 (may be NULL) is what the backward takes.  lengths [B] int32 or NULL:
  * row b has lengths[b] tokens (clamped to [0, T]); its later outputs are zero and its
- * later inputs are not read.  D a multiple of 8 up to 128, sinks <= 64, scale > 0; q, k, v
- * and o aligned to 16 bytes.  An infinity or NaN in k or v of a token that a query does
- * not see may still reach that query where both fall into one tile of 64 keys.
+ * later inputs are not used.  D a multiple of 8 up to 128, sinks <= 64, scale > 0; q, k, v
+ * and o aligned to 16 bytes.
+ *
+ * 0 times infinity or NaN is NaN, so one in v of a token that a query does not see may still
+ * reach that query: where the token shares a tile with one that any of the query's aligned 32
+ * sees.  Tiles are 32 entries of a list, the sinks and then the window of the query's aligned
+ * 128, so a sink and a token of the window may share one.  In the backward the same holds for k
+ * (towards dq), and for q and dout of a query that does not see a token (towards dk and dv) where
+ * one of its tile of 32 queries sees one of the token's aligned 32.  Where D is neither 64 nor
+ * 128, an infinity in k or dout may count as NaN.
  */
 int hattn_sliding_fwd(const void* q, const void* k, const void* v, const int* lengths,
                       const long long* strides, void* o, float* lse, int B, int T, int H, int G,

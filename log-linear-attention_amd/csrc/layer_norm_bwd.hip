@@ -5,8 +5,8 @@
 // is the gradient of x and of the residual.  Each wave keeps its columns' parameter
 // sums in registers over all its rows; they are joined per workgroup in LDS and
 // written as one partial row, and a second kernel adds the partial rows in a fixed
-// order, so that no atomic decides the result.  Bound by the bytes: 111 us and 6.5 for the
-// join (4.8 TB/s) at 65536 rows of 1024 in bf16 with a residual, 51 and 5 (4.4) at 8190 rows
+// order, so that no atomic decides the result.  Bound by the bytes: 109 us and 6 for the
+// join (4.9 TB/s) at 65536 rows of 1024 in bf16 with a residual, 49 and 5 (4.6) at 8190 rows
 // of 2304 in fp32.
 #include "layer_norm_device.h"
 

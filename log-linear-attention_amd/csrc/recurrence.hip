@@ -7,17 +7,17 @@
 //   (A2, X2) o (A1, X1) = (A2 A1, A2 X1 + X2).
 //
 // A lane owns one channel in 32 bits, or two next to each other in 16 bits (where D is even):
-// a wave reads rows of 256 bytes (rows of 128 took 103 and not 93 us forward, 150 and not
-// 133 backward, at B 4, T 8192, D 2048).  A wave holds 32 or 16 tokens in registers, a
+// a wave reads rows of 256 bytes (rows of 128 take 98 and not 91 us forward, 158 and not
+// 133 backward, at B 4, T 8192, D 2048 in bf16).  A wave holds 32 or 16 tokens in registers, a
 // workgroup eight times as many (a segment); registers are held to 128, so that a second
-// workgroup on the CU loads and stores while the first waits (133 and not 162 us backward).
+// workgroup on the CU loads and stores while the first waits (the backward with one channel a
+// lane then spills 1 to 12 of them).
 //
 // Inside the workgroup the waves' maps meet in LDS; between the segments of a channel the
 // workgroup publishes its map in a word {A, X} and then walks back over the words before it
 // until one holds a state.  A segment whose state is known replaces its word by {kState, h}, so
 // the walk is short, and the data is read once and written once: bound by the bytes (forward
-// 4.3 TB/s and backward 5.0 at the shape above in bf16, forward 4.9 at B 1, T 131072, D 1024
-// in fp32).
+// 4.4 TB/s and backward 5.0 at the shape above, forward 5.6 at B 1, T 131072, D 1024 in fp32).
 //
 // A word is 64 bits wide and is written and read by one atomic access of device
 // scope, so it is its own flag: kEmpty (a NaN pattern that publish() never writes)

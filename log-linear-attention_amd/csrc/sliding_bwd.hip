@@ -11,15 +11,16 @@
 // head, each with its own partial sums in 32 bits; the near queries' sum is one more,
 // and a last kernel adds them in order.
 //
-// delta is taken from the rounded o, whose half step is a small part of dP where many keys
-// share the weight.  In a window of up to kNarrow keys, and for the first queries of any
-// (whose gradients are the largest), it is not, and there dQ's kernel first takes
-// delta = sum P dP in a pass of its own: dQ's error against 64 bits is then 1.42 times that
-// of 32-bit products rounded once, and not up to 1.9 times.
+// P and dS are rounded to the inputs' type, which the matrix instructions take: dV's error
+// against 64 bits is 1.4 times that of one rounding.  delta is taken from the rounded o, whose
+// half step is a small part of dP where many keys share the weight.  In a window of up to
+// kNarrow keys, and for the first queries of any (whose gradients are the largest), it is not,
+// and there dQ's kernel first takes delta = sum P dP in a pass of its own: dQ's error is then
+// 1.42 times that of one rounding, and not up to 1.9 times.
 //
 // Measured at B 1, T 16384, 16 heads of 128 in 4 groups, window 4096, and at B 4, T 8192, 16
-// heads of 64, window 1024: dQ 790 and 264 us (913 and 732 TFLOP/s of its three products), dK
-// and dV 1430 and 357 us (673 and 722 of its four), the sinks 30 and 26.  dQ is bound as the
+// heads of 64, window 1024: dQ 762 and 277 us (946 and 697 TFLOP/s of its three products), dK
+// and dV 1290 and 337 us (746 and 765 of its four), the sinks 30 and 26.  dQ is bound as the
 // forward is.  dK and dV hold two accumulators and two operands, 372 registers at D 128: one
 // wave a SIMD, whose products wait for its own vector instructions.
 //

@@ -6,16 +6,18 @@
 //   S^T = K Q^T,  P = exp2(c S - m),  O^T += V^T P^T,  c = scale log2(e).
 // The accumulators are rescaled only where a row's maximum has grown by more than 8
 // (powers of two) since it was last taken, so that most tiles skip that pass; P is then
-// at most 2^8, and as exact in 16 bits as one below 1.
+// at most 2^8, and as exact in 16 bits as one below 1.  P is rounded to the inputs' type, which
+// the matrix instructions take: o's error against 64 bits is 1.35 times that of one rounding.
 //
 // K and V lie in two buffers each, filled one tile ahead by asynchronous loads.  The tiles in
 // the middle of the list, which all queries of the block see whole, have a loop of their own
 // without masks.
 //
-// Tiles of 32 keys leave registers for three waves on a SIMD (D 128) or four (D 64), whose
-// products run beside each other's softmax: 570 us at B 1, T 16384, 16 heads of 128 in 4
-// groups, window 4096 (844 TFLOP/s; 636 us with tiles of 64 and two waves), 205 us at B 4,
-// T 8192, 16 heads of 64, window 1024 (628 TFLOP/s; 273 us).  The vector instructions bound it
+// Tiles of 32 keys leave registers for three waves on a SIMD (D 128: 10 registers are spilled,
+// outside the loop without masks) or four (D 64), whose products run beside each other's
+// softmax: 552 us at B 1, T 16384, 16 heads of 128 in 4 groups, window 4096 (871 TFLOP/s),
+// 210 us at B 4, T 8192, 16 heads of 64, window 1024 (613 TFLOP/s); tiles of 64 and two waves
+// take 553 and 213 us.  The vector instructions bound it
 // at D 64 (the matrix units are busy 29% of the time); at D 128 also the card's power: on
 // zeros the same instructions take a fifth less time.
 #include "sliding_device.h"

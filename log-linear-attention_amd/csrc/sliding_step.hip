@@ -12,7 +12,7 @@
 // registers, V through a buffer of the wave's own in LDS, both one tile ahead, and no wave
 // waits for another before the end.
 //
-// 150 us at B 64, 32 heads of 128 in 8 groups, window 4096, 9000 tokens seen at most: 5.6 TB/s.
+// P is rounded to the inputs' type, as in the forward.  150 us at B 64, 32 heads of 128 in 8 groups, window 4096, 9000 tokens seen at most: 5.6 TB/s.
 //
 //   S^T[slot][head] = K Q^T,  P = exp2(c S - m),  O^T[d][head] += V^T P^T
 // (16x16x32 MFMAs in the layouts of common.h).  The new token is read from the inputs, by

@@ -124,7 +124,7 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     bytes are read in place).  Query t sees key s where s <= t and (t - s < window or
     s < sinks); sinks <= 64.  ``scale`` defaults to D ** -0.5.  ``lengths`` [B] (int32 or
     int64, on the device) are the tokens of each row of a padded batch: outputs and
-    gradients past them are zero, inputs past them are not read.  Returns o [B, T, H, D].
+    gradients past them are zero, inputs past them are not used.  Returns o [B, T, H, D].
 
     Scores, softmax and sums are fp32; the probabilities and the gradients of the scores are
     rounded to the inputs' dtype between the products.  Gradients are summed in a fixed order.
