@@ -729,7 +729,8 @@ int hattn_gated_recurrence_step(float* state, const void* x, const void* g, void
  * q [B, T, H, D], k, v [B, T, G, D] with G dividing H (head h reads group h / (H / G)), in
  * BF16 or FP16; strides: batch, token and head strides of q, then k, then v, in elements,
  * each a multiple of 8 (the last dimension is contiguous); o [B, T, H, D] contiguous;
- * lse [B, H, T] fp32 (may be NULL) is what the backward takes.  lengths [B] int32 or NULL:
+ * lse [B, H, T] fp32 (may be NULL) is what the backward takes (sizes that the backward would
+ * refuse are refused with it).  lengths [B] int32 or NULL:
  * row b has lengths[b] tokens (clamped to [0, T]); its later outputs are zero and its
  * later inputs are not used.  D a multiple of 8 up to 128, sinks <= 64, scale > 0; q, k, v
  * and o aligned to 16 bytes.
