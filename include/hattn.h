@@ -778,6 +778,78 @@ int hattn_sliding_step(const void* q, const void* k, const void* v, void* k_cach
                        int* counts, void* o, int B, int H, int G, int D, int window, int sinks,
                        float scale, int dtype, void* ws, size_t ws_bytes, void* stream);
 
+/*
+ * Global attention of a hybrid stack, next to the log-linear scans: rotary positions, a cache of
+ * keys and values in 8 bits, and attention over it.  No counterpart in the reference.
+ * Invalid sizes are HATTN_ERR_VALUE, sizes and types outside what is built
+ * HATTN_ERR_NOT_IMPLEMENTED, and so are sizes whose launch would have 2^32 threads or more.
+ */
+
+/*
+ * Rotary positions of q [B, T, H, D] and k [B, T, G, D] (G may be 0, with k and k_out NULL), in
+ * `dtype`: each pair (a, b) of the first 2 pairs elements of a head becomes
+ *   scale (a cos - b sin),  scale (a sin + b cos),  angle = position * freqs[i],
+ * the others are copied.  Pairs are (i, i + pairs), or with `interleaved` (2 i, 2 i + 1).
+ * strides: batch, token and head strides of q, then k, in elements (the last dimension is
+ * contiguous); q_out, k_out contiguous.  freqs [pairs] fp32, or fp64 with freqs64; positions:
+ * int32, or int64 with positions64, of batch b and token t at position_strides[0] * b +
+ * position_strides[1] * t; with per_row of b's first token, the others follow; NULL: token t is at
+ * t.  The angle is taken in 64 bits.  inverse: the rotation back, which is the backward.
+ * 2 pairs <= D <= 512; each element is aligned to its size.
+ */
+int hattn_rotary(const void* q, const void* k, const long long* strides, void* q_out, void* k_out,
+                 const void* freqs, int freqs64, const void* positions, int positions64,
+                 const long long* position_strides, int per_row, int B, int T, int H, int G, int D,
+                 int pairs, int interleaved, float scale, int inverse, int dtype, void* stream);
+
+/*
+ * The cache in 8 bits: k_codes, v_codes [B, G, capacity, D] in e4m3, k_scale, v_scale
+ * [B, G, capacity / 64] fp32, counts [B] int32 (tokens that each row has had), all contiguous,
+ * capacity a multiple of 64 up to 2^30, D a multiple of 16 up to 128, codes aligned to 16 bytes.
+ * Token s of a row is its code times the scale of block s / 64.  A scale is 2^e with the
+ * least e >= -100 for which 448 * 2^e holds every finite value of the block's tokens, e <= 119
+ * (7 for fp16; larger values become +-448 * 2^e); infinities and NaN are stored as NaN.  A block that
+ * gets a larger value later gets a larger scale, and its older codes are rounded again (those that
+ * fall below 2^-6; the others are exact).
+ *
+ * append: tokens k, v [B, T, G, D] (strides: batch, token, head of k, then v, in elements,
+ * multiples of 8; aligned to 16 bytes) in BF16 or FP16 enter after those that are there, of row b
+ * the first lengths[b] (clamped to [0, T]; NULL: T).  counts advance on the device, past the capacity
+ * too: those tokens are not stored.  A count may be set back: what is there stays usable up to it.
+ *
+ * read: slots [start, start + n) as k, v [B, n, G, D] contiguous, in any dtype, zero where a
+ * row has no token.
+ */
+int hattn_quant_cache_append(const void* k, const void* v, const int* lengths,
+                             const long long* strides, void* k_codes, void* v_codes, float* k_scale,
+                             float* v_scale, int* counts, int B, int T, int G, int D, int capacity,
+                             int dtype, void* stream);
+int hattn_quant_cache_read(const void* k_codes, const void* v_codes, const float* k_scale,
+                           const float* v_scale, const int* counts, void* k, void* v, int B, int G,
+                           int D, int capacity, int start, int n, int dtype, void* stream);
+
+/*
+ * Attention over it: q [B, T, H, D] in BF16 or FP16 (strides: batch, token, head) are queries of the
+ * last tokens of each row: query t of row b sees the slots s <= counts[b] - lengths[b] + t
+ * (lengths as above).  o [B, T, H, D] contiguous = softmax(scale q k^T) v over the cache's
+ * values; zero for t >= lengths[b] and where a query sees nothing, NaN in rows whose count has
+ * passed the capacity.  A NaN in v of a token may reach queries before it that share a tile of 64 tokens.
+ * step: one token a row, k, v [B, G, D], q, o [B, H, D] (strides as of T = 1: batch, token, head
+ * of q, k, v): append, then attention.  Both: workspace
+ * hattn_quant_cache_attention_workspace(B, T, ..) bytes (T = 1 for the step), aligned to 16,
+ * one for each call that may overlap.
+ */
+size_t hattn_quant_cache_attention_workspace(int B, int T, int H, int G, int D, int capacity);
+int hattn_quant_cache_attention(const void* q, const int* lengths, const long long* strides,
+                                const void* k_codes, const void* v_codes, const float* k_scale,
+                                const float* v_scale, const int* counts, void* o, int B, int T, int H,
+                                int G, int D, int capacity, float scale, int dtype, void* ws,
+                                size_t ws_bytes, void* stream);
+int hattn_quant_cache_step(const void* q, const void* k, const void* v, const long long* strides,
+                           void* k_codes, void* v_codes, float* k_scale, float* v_scale, int* counts,
+                           void* o, int B, int H, int G, int D, int capacity, float scale, int dtype,
+                           void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,231 @@
+// A cache of keys and values in 8 bits: tokens entering it and coming back.
+//
+// Appending, a workgroup makes one block of 64 tokens of one head of K or V: the new tokens
+// stay in registers between the block's maximum and their codes, so that each value is read
+// once and each code written once, which bounds it.  Where the block has older tokens and its
+// scale grows, their codes are made again.
+#include "quant_device.h"
+
+namespace hattn {
+
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) x = max(x, (unsigned)__shfl_xor((int)x, k, 64));
+  return x;
+}
+
+// The larger of the halves' finite magnitudes.
+template <typename E>
+__device__ __forceinline__ unsigned top2(unsigned x) {
+  return max(finite_bits<E>(x & 0xffff), finite_bits<E>(x >> 16));
+}
+template <typename E>
+__device__ __forceinline__ unsigned top8(uint4 x) {
+  return max(max(top2<E>(x.x), top2<E>(x.y)), max(top2<E>(x.z), top2<E>(x.w)));
+}
+
+// 2^PC lanes for the 8-element pieces of a token.
+template <typename E, int PC>
+__global__ __launch_bounds__(256) void quant_append_kernel(QuantArgs p) {
+  constexpr int ROWS = 256 >> PC, N = ROWS >= kQuantBlock ? 1 : kQuantBlock / ROWS;
+  __shared__ unsigned tops[4];
+  long item = blockIdx.x;
+  const bool isv = item & 1;
+  item >>= 1;
+  const int j = item % p.blocks;
+  const int bg = (int)(item / p.blocks), b = bg / p.G, g = bg % p.G;
+  const int n0 = max(p.counts[b], 0);
+  const int fresh = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  const long first = ((long)(n0 / kQuantBlock) + j) * kQuantBlock;  // the block's first slot
+  const long end = min((long)n0 + fresh, (long)p.cap);              // of the tokens that are kept
+  if (first >= end || n0 >= end) return;
+  const int lo = (int)max((long)n0 - first, 0L), hi = (int)min(end - first, (long)kQuantBlock);
+  float* scale = (isv ? p.vs : p.ks) + (long)bg * (p.cap / kQuantBlock) + first / kQuantBlock;
+  unsigned char* codes = (isv ? p.vc : p.kc) + ((long)bg * p.cap + first) * p.D;
+  const long st = isv ? p.vt : p.kt;
+  const __bf16* x = (const __bf16*)(isv ? p.v : p.k) + b * (isv ? p.vb : p.kb) +
+                    g * (isv ? p.vh : p.kh) + (first - n0) * st;  // row 0 of the block
+  const int d = 8 * (threadIdx.x & ((1 << PC) - 1)), row0 = threadIdx.x >> PC;
+
+  const float was = lo > 0 ? *scale : 0.f;
+  uint4 y[N];
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int row = row0 + i * ROWS;
+    y[i] = row >= lo && row < hi && d < p.D ? *(const uint4*)(x + row * st + d) : uint4{};
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = max(top, top8<E>(y[i]));
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+  const float now = fmaxf(power(scale_exponent<E>(top)), was), inverse = 1.f / now;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int row = row0 + i * ROWS;
+    if (row >= lo && row < hi && d < p.D)
+      *(uint2*)(codes + row * p.D + d) = codes8<E>(y[i], inverse);
+  }
+  if (threadIdx.x == 0) *scale = now;
+  if (lo > 0 && now > was) {
+    const float ratio = was / now;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row = row0 + i * ROWS;
+      if (row < lo && d < p.D) {
+        uint2* at = (uint2*)(codes + row * p.D + d);
+        const uint2 c = *at;
+        *at = uint2{rescale4(c.x, ratio), rescale4(c.y, ratio)};
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void quant_advance_kernel(QuantArgs p) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= p.B) return;
+  const int fresh = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+  p.counts[b] = (int)min((long)max(p.counts[b], 0) + fresh, 0x7fffffffL);
+}
+
+// One token: a workgroup makes a row's codes of all heads, a wave one head of K or V at a time,
+// and then advances the row's count, which no other workgroup reads.
+template <typename E>
+__global__ __launch_bounds__(1024) void quant_token_kernel(QuantArgs p) {
+  const int b = blockIdx.x, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int n0 = max(p.counts[b], 0);
+  if (n0 < p.cap) {
+    const int lo = n0 % kQuantBlock, first = n0 - lo;
+    for (int i = wave; i < 2 * p.G; i += waves) {
+      const bool isv = i & 1;
+      const int g = i >> 1;
+      const long bg = (long)b * p.G + g;
+      float* scale = (isv ? p.vs : p.ks) + bg * (p.cap / kQuantBlock) + first / kQuantBlock;
+      unsigned char* codes = (isv ? p.vc : p.kc) + (bg * p.cap + first) * p.D;
+      const __bf16* x = (const __bf16*)(isv ? p.v : p.k) + b * (isv ? p.vb : p.kb) +
+                        g * (isv ? p.vh : p.kh);
+      const float was = lo > 0 ? *scale : 0.f;
+      const bool mine = 2 * lane < p.D;
+      const unsigned y = mine ? *(const unsigned*)(x + 2 * lane) : 0;
+      const float now = fmaxf(power(scale_exponent<E>(wave_max(top2<E>(y)))), was);
+      const int c = codes2<E, false>(y, 1.f / now, 0);
+      if (mine) *(unsigned short*)(codes + lo * p.D + 2 * lane) = (unsigned short)c;
+      if (lane == 0) *scale = now;
+      if (lo > 0 && now > was) {
+        const float ratio = was / now;
+        for (int at = 16 * lane; at < lo * p.D; at += 1024) {
+          uint4 old = *(const uint4*)(codes + at);
+          old = uint4{rescale4(old.x, ratio), rescale4(old.y, ratio), rescale4(old.z, ratio),
+                      rescale4(old.w, ratio)};
+          *(uint4*)(codes + at) = old;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) p.counts[b] = min(n0, 0x7ffffffe) + 1;
+}
+
+// 2^PC lanes for the 16-element pieces of a token; a workgroup has one block of a head of K or V,
+// so that its scale is one number.
+template <typename T, int PC>
+__global__ __launch_bounds__(256) void quant_read_kernel(QuantArgs p) {
+  constexpr int ROWS = 256 >> PC, N = ROWS >= kQuantBlock ? 1 : kQuantBlock / ROWS;
+  long item = blockIdx.x;
+  const bool isv = item & 1;
+  item >>= 1;
+  const int j = item % p.blocks;
+  const int bg = (int)(item / p.blocks), b = bg / p.G, g = bg % p.G;
+  const int first = (p.start / kQuantBlock + j) * kQuantBlock;
+  const int count = p.counts[b], end = p.start + p.n;
+  const float scale = (isv ? p.vs : p.ks)[(long)bg * (p.cap / kQuantBlock) + first / kQuantBlock];
+  const unsigned char* codes = (isv ? p.vc : p.kc) + (long)bg * p.cap * p.D;
+  T* out = (T*)(isv ? p.vo : p.ko);
+  const int d = 16 * (threadIdx.x & ((1 << PC) - 1)), row0 = threadIdx.x >> PC;
+  if (d >= p.D) return;
+  uint4 x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int slot = first + row0 + i * ROWS;
+    x[i] = slot >= p.start && slot < end && slot < count && row0 + i * ROWS < kQuantBlock
+               ? *(const uint4*)(codes + (long)slot * p.D + d) : uint4{};
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int slot = first + row0 + i * ROWS;
+    if (slot < p.start || slot >= end || row0 + i * ROWS >= kQuantBlock) continue;
+    struct alignas(16) Out {
+      T v[16];
+    } y;
+    const unsigned w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false);
+      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
+      const float f[4] = {lo[0], lo[1], hi[0], hi[1]};
+      // slots that hold no token are zero whatever the scale there
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y.v[4 * k + e] = from_f32<T>(slot < count ? f[e] * scale : 0.f);
+    }
+    *(Out*)(out + (((long)b * p.n + slot - p.start) * p.G + g) * p.D + d) = y;
+  }
+}
+
+}  // namespace hattn
+
+hipError_t hattn_quant_append_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
+  using namespace hattn;
+  const dim3 grid((unsigned)((long)p.B * p.G * p.blocks * 2));
+#define GO(E, PC) hipLaunchKernelGGL((quant_append_kernel<E, PC>), grid, dim3(256), 0, stream, p)
+#define PICK(E)             \
+  if (p.D <= 16) GO(E, 1);  \
+  else if (p.D <= 32) GO(E, 2); \
+  else if (p.D <= 64) GO(E, 3); \
+  else GO(E, 4);
+  if (dtype == 1) {
+    PICK(_Float16)
+  } else {
+    PICK(__bf16)
+  }
+#undef PICK
+#undef GO
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  hipLaunchKernelGGL(quant_advance_kernel, dim3((unsigned)((p.B + 255) / 256)), dim3(256), 0, stream,
+                     p);
+  return hipGetLastError();
+}
+
+hipError_t hattn_quant_token_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
+  using namespace hattn;
+  const dim3 grid((unsigned)p.B), block(64 * (2 * p.G < 16 ? 2 * p.G : 16));
+  if (dtype == 1)
+    hipLaunchKernelGGL((quant_token_kernel<_Float16>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((quant_token_kernel<__bf16>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t hattn_quant_read_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
+  using namespace hattn;
+  const dim3 grid((unsigned)((long)p.B * p.G * p.blocks * 2));
+#define GO(T, PC) hipLaunchKernelGGL((quant_read_kernel<T, PC>), grid, dim3(256), 0, stream, p)
+#define PICK(T)             \
+  if (p.D <= 16) GO(T, 0);  \
+  else if (p.D <= 32) GO(T, 1); \
+  else if (p.D <= 64) GO(T, 2); \
+  else GO(T, 3);
+  if (dtype == 0) {
+    PICK(__bf16)
+  } else if (dtype == 1) {
+    PICK(_Float16)
+  } else {
+    PICK(float)
+  }
+#undef PICK
+#undef GO
+  return hipGetLastError();
+}

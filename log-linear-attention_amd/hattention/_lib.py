@@ -95,6 +95,12 @@ SIGNATURES = [
     ("hattn_sliding_cache_fill", _I, [_P] * 7 + [_I] * 7 + [_P]),
     ("hattn_sliding_step_workspace", _S, [_I] * 6),
     ("hattn_sliding_step", _I, [_P] * 7 + [_I] * 6 + [ctypes.c_float, _I, _P, _S, _P]),
+    ("hattn_rotary", _I, [_P] * 6 + [_I, _P, _I, _P] + [_I] * 8 + [ctypes.c_float, _I, _I, _P]),
+    ("hattn_quant_cache_append", _I, [_P] * 9 + [_I] * 6 + [_P]),
+    ("hattn_quant_cache_read", _I, [_P] * 7 + [_I] * 7 + [_P]),
+    ("hattn_quant_cache_attention_workspace", _S, [_I] * 6),
+    ("hattn_quant_cache_attention", _I, [_P] * 9 + [_I] * 6 + [ctypes.c_float, _I, _P, _S, _P]),
+    ("hattn_quant_cache_step", _I, [_P] * 10 + [_I] * 5 + [ctypes.c_float, _I, _P, _S, _P]),
 ]
 
 _lock = threading.Lock()

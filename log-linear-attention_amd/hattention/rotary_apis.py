@@ -1,0 +1,174 @@
+"""Rotary positions of queries and keys (MI355X): training and decode.
+
+What a hybrid stack's attention layers (``sliding_apis``, ``quant_cache_apis``) apply to q and
+k before the scores.  One launch for both tensors, forward and backward (libhattn_hip.so:
+``hattn_rotary``).  No counterpart in the reference.
+"""
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from hattention import _lib
+
+MAX_D = 512
+LAYOUTS = ("half", "interleaved")
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] = None,
+                       factor: float = 1.0, original_length: Optional[int] = None,
+                       fast: float = 32.0, slow: float = 1.0,
+                       device="cuda") -> Tuple[torch.Tensor, float]:
+    """(freqs, scale) for :func:`rotary_embedding`: the dim / 2 frequencies base ** (-2 i / dim) in
+    radians a token (fp64, on ``device``), for contexts ``factor`` times as long as trained with
+    where ``scaling`` is
+
+    * ``"linear"``: positions divided by ``factor``;
+    * ``"ntk"``: a base for which the slowest frequency is divided by ``factor`` and the fastest
+      stays, base * factor ** (dim / (dim - 2));
+    * ``"yarn"`` (Peng et al. 2023, "YaRN: Efficient Context Window Extension of Large Language
+      Models"): with r the turns of a frequency within ``original_length`` tokens, frequencies of
+      r >= ``fast`` stay, those of r <= ``slow`` are divided by ``factor``, those between are mixed
+      of both, linearly in r; scale = 1 + 0.1 log(factor).  In the others scale = 1.
+    """
+    if dim < 2 or dim % 2 != 0:
+        raise ValueError(f"dim={dim} is not a positive even number")
+    if not 1.0 < base < math.inf:
+        raise ValueError(f"base={base}")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling={scaling!r}")
+    if not 1.0 <= factor < math.inf:
+        raise ValueError(f"factor={factor} below 1")
+    n, scale = dim // 2, 1.0
+    if scaling == "ntk":
+        if dim == 2:
+            raise ValueError("dim=2 has one frequency, which \"ntk\" keeps")
+        base = base * factor ** (dim / (dim - 2))
+    freqs = [base ** (-2.0 * i / dim) for i in range(n)]
+    if scaling == "linear":
+        freqs = [f / factor for f in freqs]
+    elif scaling == "yarn":
+        if original_length is None or original_length < 1:
+            raise ValueError("\"yarn\" needs original_length")
+        if not 0.0 < slow < fast:
+            raise ValueError(f"fast={fast}, slow={slow}")
+        for i, f in enumerate(freqs):
+            turns = original_length * f / (2.0 * math.pi)
+            stay = min(max((turns - slow) / (fast - slow), 0.0), 1.0)
+            freqs[i] = f * stay + f / factor * (1.0 - stay)
+        scale = 1.0 + 0.1 * math.log(factor)
+    return torch.tensor(freqs, dtype=torch.float64, device=device), scale
+
+
+def _strides(t) -> list:
+    """Batch, token and head strides (0 where the size is 1: torch leaves such a stride at any
+    value)."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())]
+
+
+def _launch(q, k, freqs, positions, interleaved, scale, inverse):
+    B, T, H, D = q.shape
+    q = q if q.stride(3) == 1 or D == 1 else q.contiguous()
+    qo, ko, G = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device), None, 0
+    strides = _strides(q)
+    if k is not None:
+        G = k.shape[2]
+        k = k if k.stride(3) == 1 or D == 1 else k.contiguous()
+        ko = torch.empty(B, T, G, D, dtype=q.dtype, device=q.device)
+        strides += _strides(k)
+    else:
+        strides += [0, 0, 0]
+    at = None
+    if positions is not None:
+        at = [s if n > 1 else 0 for n, s in zip(positions.shape, positions.stride())] + [0]
+    _lib.launch(q.device, _lib.load().hattn_rotary, q.data_ptr(), _lib.ptr(k),
+                (ctypes.c_longlong * 6)(*strides), qo.data_ptr(), _lib.ptr(ko), freqs.data_ptr(),
+                freqs.dtype == torch.float64, _lib.ptr(positions),
+                positions is not None and positions.dtype == torch.int64,
+                (ctypes.c_longlong * 2)(*at[:2]) if at else None,
+                positions is not None and positions.dim() == 1, B, T, H, G, D, freqs.shape[0],
+                interleaved, scale, inverse, _lib.dtype_code(q))
+    return qo, ko
+
+
+class RotaryFunction(torch.autograd.Function):
+    """(q, k) of :func:`rotary_embedding`; the backward turns the gradients back."""
+
+    @staticmethod
+    def forward(ctx, q, k, freqs, positions, interleaved, scale):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(freqs, positions)
+        ctx.cfg = interleaved, scale
+        return _launch(q, k, freqs, positions, interleaved, scale, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        freqs, positions = ctx.saved_tensors
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        if dq is not None:
+            dq, dk = _launch(dq, dk, freqs, positions, *ctx.cfg, True)
+        elif dk is not None:
+            dk, _ = _launch(dk, None, freqs, positions, *ctx.cfg, True)
+        return dq, dk, None, None, None, None
+
+
+def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor,
+                     positions: Optional[torch.Tensor] = None, layout: str = "half",
+                     scale: float = 1.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """q and k turned by their positions: in each head, pair i of the first 2 * len(freqs)
+    elements is rotated by position * freqs[i] and multiplied by ``scale``; the others stay.
+
+    q [B, T, H, D] and k [B, T, G, D] (or None), or one token a row, [B, H, D] and [B, G, D], in bf16,
+    fp16 or fp32, of any strides; D <= 512.  freqs [n], fp32 or fp64 (:func:`rotary_frequencies`);
+    2 n <= D.  ``layout`` "half" pairs elements i and i + n, "interleaved" 2 i and 2 i + 1.
+    ``positions`` (int32 or int64, on the device): [B], of each row's first token, or [B, T], of every
+    token; None: 0 to T - 1 (one token a row needs [B]).  Returns (q, k), contiguous; gradients
+    reach q and k.
+
+    Angles are taken and reduced in 64 bits, sines and products in 32, at any position.
+    """
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout={layout!r}: one of {LAYOUTS}")
+    one = q.dim() == 3
+    if q.dim() not in (3, 4) or (k is not None and k.dim() != q.dim()):
+        raise ValueError("q and k must be [B, T, heads, D] or [B, heads, D]")
+    if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]):
+        raise ValueError(f"shapes of q {tuple(q.shape)}, k {tuple(k.shape)}")
+    if 0 in q.shape or (k is not None and 0 in k.shape):
+        raise ValueError("empty tensor")
+    if k is not None and k.dtype != q.dtype:
+        raise ValueError("q and k must have one dtype")
+    _lib.dtype_code(q)
+    D = q.shape[-1]
+    if freqs.dim() != 1 or not 1 <= freqs.shape[0] <= D // 2:
+        raise ValueError(f"freqs {tuple(freqs.shape)} for heads of {D}")
+    if freqs.dtype not in (torch.float32, torch.float64):
+        raise NotImplementedError(f"freqs in {freqs.dtype}")
+    if D > MAX_D:
+        raise NotImplementedError(f"D={D} above {MAX_D}")
+    if not math.isfinite(scale) or abs(scale) > 1e30:
+        raise ValueError(f"scale={scale}")
+    B = q.shape[0]
+    if positions is not None:
+        if positions.shape not in ((B,), () if one else tuple(q.shape[:2])):
+            raise ValueError(f"positions {tuple(positions.shape)} for q {tuple(q.shape)}")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise NotImplementedError(f"positions in {positions.dtype}")
+    elif one:
+        raise ValueError("one token a row needs positions [B]")
+    _lib.require_device(q, k, freqs, positions)
+    freqs = freqs.detach().contiguous()
+    if one:
+        q, k = q.unsqueeze(1), k.unsqueeze(1) if k is not None else None
+    args = q, k, freqs, positions, layout == "interleaved", float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        q, k = RotaryFunction.apply(*args)
+    else:
+        q, k = _launch(*args, False)
+    if one:
+        q, k = q.squeeze(1), k.squeeze(1) if k is not None else None
+    return q, k
