@@ -792,15 +792,16 @@ int hattn_sliding_step(const void* q, const void* k, const void* v, void* k_cach
  * the others are copied.  Pairs are (i, i + pairs), or with `interleaved` (2 i, 2 i + 1).
  * strides: batch, token and head strides of q, then k, in elements (the last dimension is
  * contiguous); q_out, k_out contiguous.  freqs [pairs] fp32, or fp64 with freqs64; positions:
- * int32, or int64 with positions64, of batch b and token t at position_strides[0] * b +
- * position_strides[1] * t; with per_row of b's first token, the others follow; NULL: token t is at
+ * int32, or int64 with positions64, of batch b and token t at position_batch * b +
+ * position_token * t; with per_row of b's first token, the others follow; NULL: token t is at
  * t.  The angle is taken in 64 bits.  inverse: the rotation back, which is the backward.
  * 2 pairs <= D <= 512; each element is aligned to its size.
  */
 int hattn_rotary(const void* q, const void* k, const long long* strides, void* q_out, void* k_out,
                  const void* freqs, int freqs64, const void* positions, int positions64,
-                 const long long* position_strides, int per_row, int B, int T, int H, int G, int D,
-                 int pairs, int interleaved, float scale, int inverse, int dtype, void* stream);
+                 long long position_batch, long long position_token, int per_row, int B, int T, int H,
+                 int G, int D, int pairs, int interleaved, float scale, int inverse, int dtype,
+                 void* stream);
 
 /*
  * The cache in 8 bits: k_codes, v_codes [B, G, capacity, D] in e4m3, k_scale, v_scale

@@ -101,7 +101,7 @@ int attention_checks(int B, int T, int H, int G, int D, int capacity, float scal
   if ((double)T * (H / G) > (double)(INT_MAX / 2))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "T=%d H=%d: 2^30 queries of a key head or more", T, H);
   const Cut c = cut(B, T, H, G, capacity);
-  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) || !fits((double)B * T * H, 128))
+  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) || !fits((double)B * T * H, 256))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: 2^24 workgroups or more", B, T, H);
   return HATTN_OK;
 }
@@ -139,8 +139,9 @@ extern "C" {
 
 int hattn_rotary(const void* q, const void* k, const long long* strides, void* q_out, void* k_out,
                  const void* freqs, int freqs64, const void* positions, int positions64,
-                 const long long* position_strides, int per_row, int B, int T, int H, int G, int D,
-                 int pairs, int interleaved, float scale, int inverse, int dtype, void* stream) {
+                 long long position_batch, long long position_token, int per_row, int B, int T, int H,
+                 int G, int D, int pairs, int interleaved, float scale, int inverse, int dtype,
+                 void* stream) {
   if (B <= 0 || T <= 0 || H <= 0 || G < 0 || D <= 0 || pairs <= 0)
     return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (2LL * pairs > D) return fail(HATTN_ERR_VALUE, "%d pairs in heads of %d", pairs, D);
@@ -149,7 +150,7 @@ int hattn_rotary(const void* q, const void* k, const long long* strides, void* q
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "dtype code %d", dtype);
   if (D > kRotaryMaxD) return fail(HATTN_ERR_NOT_IMPLEMENTED, "D=%d above %d", D, kRotaryMaxD);
   if ((double)H + G > 1 << 20) return fail(HATTN_ERR_NOT_IMPLEMENTED, "H=%d G=%d: above 2^20", H, G);
-  if (!q || !q_out || (G > 0 && (!k || !k_out)) || !strides || !freqs || (positions && !position_strides))
+  if (!q || !q_out || (G > 0 && (!k || !k_out)) || !strides || !freqs)
     return fail(HATTN_ERR_VALUE, "null tensor pointer");
   const int bytes = dtype == HATTN_FP32 ? 4 : 2, vec = 16 / bytes;
   if (!aligned({q, q_out, G > 0 ? k : q, G > 0 ? k_out : q_out}, bytes) ||
@@ -170,22 +171,20 @@ int hattn_rotary(const void* q, const void* k, const long long* strides, void* q
   }
   p.freqs = freqs; p.freq64 = freqs64;
   p.pos = positions; p.pos64 = positions64;
-  if (positions) {
-    p.pb = position_strides[0];
-    p.pt = position_strides[1];
-  }
+  p.pb = position_batch; p.pt = position_token;
   p.from = per_row;
   p.N = (long)B * T;
   p.T = T; p.D = D; p.pairs = pairs;
   p.scale = scale;
   p.sign = inverse ? -1.f : 1.f;
-  const int v = rotary_vec(bytes, wide), lanes = pairs / v + (D - 2 * pairs + 2 * v - 1) / (2 * v);
+  const int v = rotary_vec(bytes, wide), lanes = pairs / v + ((D - 2 * pairs) / v + 1) / 2;
   p.cols = 1;
   while (p.cols < lanes) p.cols *= 2;
-  // about eight turns of a workgroup's lanes, but at least 1024 workgroups where the tokens allow
-  // it, and sines of at most 8 KB
+  // One round of kAhead heads a lane, so that many workgroups, in their several phases, share a CU
+  // (4 x 8192 tokens of 32 heads of 64 in bf16: 55 us; with twice the tokens 60, half of them 56),
+  // but at least 1024 workgroups where the tokens allow it, and sines of at most 8 KB.
   const long heads = (long)H + G;
-  p.tokens = (int)std::max(1L, std::min({2048 / (heads * p.cols), (long)(1024 / pairs), p.N / 1024}));
+  p.tokens = (int)std::max(1L, std::min({512 / (heads * p.cols), (long)(1024 / pairs), p.N / 1024}));
   if (!fits(std::ceil((double)p.N / p.tokens), 256))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d: 2^24 workgroups or more", B, T);
   return check_hip(hattn_rotary_launch(p, dtype, interleaved != 0, wide, (hipStream_t)stream),

@@ -216,22 +216,24 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
   }
 }
 
-// Joins a query's partial results, those of the parts that have tokens; one thread an element.
+// Joins a query's partial results, those of the parts that have tokens: groups of lanes that hold
+// 4 elements each take every n-th part, and the groups' sums meet in LDS, in order.
 template <typename E>
-__global__ __launch_bounds__(128) void quant_join_kernel(QuantArgs p) {
+__global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
   __shared__ float share[kQuantSplits];
+  __shared__ floatx4 sums[256];
   const long query = blockIdx.x, bt = query / p.H;
   const int b = (int)(bt / p.T), t = (int)(bt - (long)b * p.T), lane = threadIdx.x & 63;
   const QuantRow row(p, b);
   __bf16* o = (__bf16*)p.o + query * p.D;
-  const int d = threadIdx.x;
   if (row.end(t) == 0) {  // it sees nothing
-    if (d < p.D) o[d] = to16<E>(row.full && t < row.fresh ? __builtin_nanf("") : 0.f);
+    const float none = row.full && t < row.fresh ? __builtin_nanf("") : 0.f;
+    if (threadIdx.x < p.D) o[threadIdx.x] = to16<E>(none);
     return;
   }
   const int each = part_tokens(row.n, p.splits), live = (row.n + each - 1) / each;
   const float* stat = p.stat + query * p.splits * 2;
-  // both waves take the maximum and the sum, a part a lane
+  // every wave takes the maximum and the sum, a part a lane
   float top = -INFINITY, sum = 0.f;
   for (int s = lane; s < live; s += 64) top = fmaxf(top, stat[2 * s]);
 #pragma unroll
@@ -244,16 +246,26 @@ __global__ __launch_bounds__(128) void quant_join_kernel(QuantArgs p) {
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k, 64);
   __syncthreads();
-  if (d >= p.D) return;
-  const float* part = p.part + query * p.splits * p.D + d;
-  float x = 0.f, y[8];
-  for (int s = 0; s < live; s += 8) {
+  const int pieces = p.D / 4, groups = 256 / pieces;
+  const int group = threadIdx.x / pieces, c = threadIdx.x - group * pieces;
+  floatx4 x = zero4();
+  if (group < groups) {
+    const float* part = p.part + query * p.splits * p.D + 4 * c;
+#pragma unroll 4
+    for (int s = group; s < live; s += groups) {
+      const floatx4 y = *(const floatx4*)(part + (long)s * p.D);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) y[u] = s + u < live ? part[(long)(s + u) * p.D] * share[s + u] : 0.f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) x += y[u];
+      for (int i = 0; i < 4; ++i) x[i] = fmaf(y[i], share[s], x[i]);
+    }
+    sums[threadIdx.x] = x;
   }
-  o[d] = to16<E>(x / sum);
+  __syncthreads();
+  if (group != 0) return;
+  for (int s = 1; s < min(groups, live); ++s) x += sums[s * pieces + c];
+  bf16x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = to16<E>(x[i] / sum);
+  *(bf16x4*)(o + 4 * c) = y;
 }
 
 }  // namespace hattn
@@ -277,8 +289,8 @@ hipError_t hattn_quant_join_launch(const QuantArgs& p, int dtype, hipStream_t st
   using namespace hattn;
   const dim3 grid((unsigned)((long)p.B * p.T * p.H));
   if (dtype == 1)
-    hipLaunchKernelGGL((quant_join_kernel<_Float16>), grid, dim3(128), 0, stream, p);
+    hipLaunchKernelGGL((quant_join_kernel<_Float16>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((quant_join_kernel<__bf16>), grid, dim3(128), 0, stream, p);
+    hipLaunchKernelGGL((quant_join_kernel<__bf16>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }

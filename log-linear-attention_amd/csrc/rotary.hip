@@ -16,6 +16,8 @@
 
 namespace hattn {
 
+constexpr int kAhead = 2;
+
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Piece {
   T v[V];
@@ -59,49 +61,60 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
 
   const int heads = p.heads[0] + p.heads[1], rot = 2 * p.pairs;
   const int col = threadIdx.x % p.cols, rows = 256 / p.cols;
-  // the lane's two pieces
-  int a, b;
-  const int turning = INTER ? rot / (2 * V) : p.pairs / V;  // lanes with pairs
+  // The lane's two pieces: each in its own half of the pairs or of what stays, so that neighbours
+  // read on; single elements that are interleaved lie together.
+  const int turning = p.pairs / V, col2 = col - turning;  // lanes with pairs
+  const int staying = ((p.D - rot) / V + 1) / 2;
   const bool turn = col < turning;
-  if (turn) {
-    a = INTER ? 2 * V * col : V * col;
-    b = INTER ? a + V : a + p.pairs;
-  } else {
-    a = rot + 2 * V * (col - turning);
-    b = a + V;
-  }
-  if (a >= p.D) return;
+  const int a = !turn ? rot + V * col2 : INTER && V == 1 ? 2 * col : V * col;
+  const int b = !turn ? a + V * staying : INTER && V == 1 ? a + 1 : a + p.pairs;
+  if (!turn && col2 >= staying) return;
   const bool two = b < p.D;
   int h = threadIdx.x / p.cols, tt = h / heads;
   h -= tt * heads;
   const int dt = rows / heads, dh = rows - dt * heads;
   typedef Piece<T, V> P;
-  for (; tt < tokens;) {
-    const int w = h >= p.heads[0], hw = w ? h - p.heads[0] : h;
-    const T* x = (const T*)p.x[w] + at[w * p.tokens + tt] + hw * p.xh[w];
-    T* y = (T*)p.y[w] + ((n0 + tt) * p.heads[w] + hw) * p.D;
-    P u = *(const P*)(x + a), v{};
-    if (two) v = *(const P*)(x + b);
-    if (turn) {
-      const float2* angle = cs + tt * p.pairs + (INTER ? a / 2 : a);
-      if constexpr (INTER && V > 1) {
+  // kAhead heads at once: their loads are in flight together
+  while (tt < tokens) {
+    P u[kAhead], v[kAhead];
+    int token[kAhead];
+    T* y[kAhead];
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-          turned(u.v[2 * i], u.v[2 * i + 1], angle[i]);
-          turned(v.v[2 * i], v.v[2 * i + 1], angle[V / 2 + i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) turned(u.v[i], v.v[i], angle[i]);
+    for (int k = 0; k < kAhead; ++k) {
+      token[k] = tt < tokens ? tt : -1;
+      u[k] = v[k] = P{};
+      if (tt < tokens) {
+        const int w = h >= p.heads[0], hw = w ? h - p.heads[0] : h;
+        const T* x = (const T*)p.x[w] + at[w * p.tokens + tt] + hw * p.xh[w];
+        y[k] = (T*)p.y[w] + ((n0 + tt) * p.heads[w] + hw) * p.D;
+        u[k] = *(const P*)(x + a);
+        if (two) v[k] = *(const P*)(x + b);
+      }
+      tt += dt;
+      h += dh;
+      if (h >= heads) {
+        h -= heads;
+        ++tt;
       }
     }
-    *(P*)(y + a) = u;
-    if (two) *(P*)(y + b) = v;
-    tt += dt;
-    h += dh;
-    if (h >= heads) {
-      h -= heads;
-      ++tt;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (token[k] < 0) break;
+      if (turn) {
+        const float2* angle = cs + token[k] * p.pairs + (INTER ? a / 2 : a);
+        if constexpr (INTER && V > 1) {
+#pragma unroll
+          for (int i = 0; i < V / 2; ++i) {
+            turned(u[k].v[2 * i], u[k].v[2 * i + 1], angle[i]);
+            turned(v[k].v[2 * i], v[k].v[2 * i + 1], angle[p.pairs / 2 + i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) turned(u[k].v[i], v[k].v[i], angle[i]);
+        }
+      }
+      *(P*)(y[k] + a) = u[k];
+      if (two) *(P*)(y[k] + b) = v[k];
     }
   }
 }

@@ -95,7 +95,7 @@ SIGNATURES = [
     ("hattn_sliding_cache_fill", _I, [_P] * 7 + [_I] * 7 + [_P]),
     ("hattn_sliding_step_workspace", _S, [_I] * 6),
     ("hattn_sliding_step", _I, [_P] * 7 + [_I] * 6 + [ctypes.c_float, _I, _P, _S, _P]),
-    ("hattn_rotary", _I, [_P] * 6 + [_I, _P, _I, _P] + [_I] * 8 + [ctypes.c_float, _I, _I, _P]),
+    ("hattn_rotary", _I, [_P] * 6 + [_I, _P, _I, _LL, _LL] + [_I] * 8 + [ctypes.c_float, _I, _I, _P]),
     ("hattn_quant_cache_append", _I, [_P] * 9 + [_I] * 6 + [_P]),
     ("hattn_quant_cache_read", _I, [_P] * 7 + [_I] * 7 + [_P]),
     ("hattn_quant_cache_attention_workspace", _S, [_I] * 6),
@@ -150,16 +150,15 @@ def require_device(*tensors) -> torch.device:
     """All tensors must live on one HIP device; the path has no CPU fallback."""
     dev = None
     for t in tensors:
-        if t is None:
+        if t is None or t.device == dev:
             continue
         if t.device.type != "cuda":
             raise RuntimeError(
                 "hattention (MI355X) runs only on HIP device tensors; got a tensor on "
                 f"{t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if dev is not None:
             raise RuntimeError("tensors on different devices")
+        dev = t.device
     return dev
 
 

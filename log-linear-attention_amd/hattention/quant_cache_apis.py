@@ -5,6 +5,7 @@ cache that keeps every token, in half the memory of 16 bits, which bounds decodi
 libhattn_hip.so's ``hattn_quant_cache_append`` / ``_read`` / ``_attention`` / ``_step``.  No
 counterpart in the reference.
 """
+import ctypes
 import functools
 from typing import Optional, Tuple
 
@@ -12,11 +13,26 @@ import torch
 
 from hattention import _lib
 from hattention.recurrence_apis import check_lengths
-from hattention.sliding_apis import _rows, _strides
 
 BLOCK = 64
 MAX_CAPACITY = 2 ** 30
 E4M3 = torch.float8_e4m3fn
+
+
+_Strides3, _Strides6, _Strides9 = (ctypes.c_longlong * n for n in (3, 6, 9))
+
+
+def _lead(t):
+    """t, or a copy, with contiguous rows that start on 16 bytes, and its batch, token and head
+    strides (0 where there is one element: torch leaves such a stride at any value)."""
+    s, n = t.stride(), t.shape
+    if len(n) == 3:  # one token a row
+        lead = s[0] if n[0] > 1 else 0, 0, s[1] if n[1] > 1 else 0
+    else:
+        lead = s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0
+    if s[-1] == 1 and t.data_ptr() % 16 == 0 and (lead[0] | lead[1] | lead[2]) % 8 == 0:
+        return t, lead
+    return _lead(t.clone(memory_format=torch.contiguous_format))
 
 
 @functools.lru_cache(maxsize=256)
@@ -115,7 +131,6 @@ def _check_queries(cache, q, scale) -> float:
     return scale
 
 
-@torch.no_grad()
 def quant_cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor,
                        lengths: Optional[torch.Tensor] = None) -> QuantCache:
     """Tokens k, v [B, T, G, D] (bf16 or fp16, any strides) enter the cache after each row's last
@@ -131,14 +146,13 @@ def quant_cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"T={T} tokens for a capacity of {cache.capacity}")
     dev = _lib.require_device(k, v, *cache._tensors())
     lengths = check_lengths(lengths, B, dev)
-    k, v = _rows(k), _rows(v)
+    (k, sk), (v, sv) = _lead(k), _lead(v)
     _lib.launch(dev, _lib.load().hattn_quant_cache_append, k.data_ptr(), v.data_ptr(),
-                _lib.ptr(lengths), _strides(k, v), *cache._ptrs(), B, T, k.shape[2], k.shape[3],
+                _lib.ptr(lengths), _Strides6(*sk, *sv), *cache._ptrs(), B, T, k.shape[2], k.shape[3],
                 cache.capacity, _lib.dtype_code(k))
     return cache
 
 
-@torch.no_grad()
 def quant_cache_read(cache: QuantCache, dtype: torch.dtype = torch.bfloat16, start: int = 0,
                      stop: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Tokens start .. stop - 1 (to the capacity without ``stop``) of every row as k, v
@@ -157,7 +171,6 @@ def quant_cache_read(cache: QuantCache, dtype: torch.dtype = torch.bfloat16, sta
     return k, v
 
 
-@torch.no_grad()
 def quant_cache_attention(cache: QuantCache, q: torch.Tensor, scale: Optional[float] = None,
                           lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of each row's last tokens over the cache, which holds them already
@@ -179,17 +192,16 @@ def quant_cache_attention(cache: QuantCache, q: torch.Tensor, scale: Optional[fl
     dev = _lib.require_device(q, *cache._tensors())
     B, T, H, D = q.shape
     lengths = check_lengths(lengths, B, dev)
-    q = _rows(q)
+    q, sq = _lead(q)
     o = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
     sizes = B, T, H, cache.k.shape[1], D, cache.capacity
     ws, ws_ptr, ws_bytes = _lib.workspace(_attention_bytes(*sizes), dev)
     _lib.launch(dev, _lib.load().hattn_quant_cache_attention, q.data_ptr(), _lib.ptr(lengths),
-                _strides(q), *cache._ptrs(), o.data_ptr(), *sizes, scale, _lib.dtype_code(q), ws_ptr,
+                _Strides3(*sq), *cache._ptrs(), o.data_ptr(), *sizes, scale, _lib.dtype_code(q), ws_ptr,
                 ws_bytes)
     return o
 
 
-@torch.no_grad()
 def quant_cache_step(cache: QuantCache, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      scale: Optional[float] = None) -> Tuple[torch.Tensor, QuantCache]:
     """One token per row: q [B, H, D], k, v [B, G, D].  The token enters the cache, and q sees it
@@ -203,11 +215,11 @@ def quant_cache_step(cache: QuantCache, q: torch.Tensor, k: torch.Tensor, v: tor
     _check_half(q, k, v)
     dev = _lib.require_device(q, k, v, *cache._tensors())
     B, H, D = q.shape
-    q, k, v = (_rows(t.unsqueeze(1)) for t in (q, k, v))
+    (q, sq), (k, sk), (v, sv) = _lead(q), _lead(k), _lead(v)
     o = torch.empty(B, H, D, dtype=q.dtype, device=dev)
     G, slots = cache.k.shape[1:3]
     ws, ws_ptr, ws_bytes = _lib.workspace(_attention_bytes(B, 1, H, G, D, slots), dev)
     _lib.launch(dev, _lib.load().hattn_quant_cache_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                _strides(q, k, v), *cache._ptrs(), o.data_ptr(), B, H, G, D, slots, scale,
+                _Strides9(*sq, *sk, *sv), *cache._ptrs(), o.data_ptr(), B, H, G, D, slots, scale,
                 _lib.dtype_code(q), ws_ptr, ws_bytes)
     return o, cache

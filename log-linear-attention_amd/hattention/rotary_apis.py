@@ -62,34 +62,44 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     return torch.tensor(freqs, dtype=torch.float64, device=device), scale
 
 
-def _strides(t) -> list:
-    """Batch, token and head strides (0 where the size is 1: torch leaves such a stride at any
-    value)."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())]
+_Strides = ctypes.c_longlong * 6
+
+
+def _lead(t):
+    """t with a contiguous last dimension, and its batch, token and head strides (0 where there is
+    one element: torch leaves such a stride at any value)."""
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
+        s = t.stride()
+    n = t.shape
+    if len(n) == 3:  # one token a row
+        return t, (s[0] if n[0] > 1 else 0, 0, s[1] if n[1] > 1 else 0)
+    return t, (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
 
 
 def _launch(q, k, freqs, positions, interleaved, scale, inverse):
-    B, T, H, D = q.shape
-    q = q if q.stride(3) == 1 or D == 1 else q.contiguous()
-    qo, ko, G = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device), None, 0
-    strides = _strides(q)
+    """(q, k) of [B, T, heads, D], or [B, heads, D], turned."""
+    q, strides = _lead(q)
+    n = q.shape
+    B, H, D = n[0], n[-2], n[-1]
+    T = n[1] if len(n) == 4 else 1
+    qo, ko, G = torch.empty(n, dtype=q.dtype, device=q.device), None, 0
     if k is not None:
-        G = k.shape[2]
-        k = k if k.stride(3) == 1 or D == 1 else k.contiguous()
-        ko = torch.empty(B, T, G, D, dtype=q.dtype, device=q.device)
-        strides += _strides(k)
-    else:
-        strides += [0, 0, 0]
-    at = None
+        k, more = _lead(k)
+        G = k.shape[-2]
+        ko = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        strides += more
+    pb = pt = per_row = wide = 0
     if positions is not None:
-        at = [s if n > 1 else 0 for n, s in zip(positions.shape, positions.stride())] + [0]
-    _lib.launch(q.device, _lib.load().hattn_rotary, q.data_ptr(), _lib.ptr(k),
-                (ctypes.c_longlong * 6)(*strides), qo.data_ptr(), _lib.ptr(ko), freqs.data_ptr(),
-                freqs.dtype == torch.float64, _lib.ptr(positions),
-                positions is not None and positions.dtype == torch.int64,
-                (ctypes.c_longlong * 2)(*at[:2]) if at else None,
-                positions is not None and positions.dim() == 1, B, T, H, G, D, freqs.shape[0],
-                interleaved, scale, inverse, _lib.dtype_code(q))
+        per_row = positions.dim() == 1
+        wide = positions.dtype == torch.int64
+        pb = positions.stride(0) if B > 1 else 0
+        pt = positions.stride(1) if not per_row and T > 1 else 0
+    _lib.launch(q.device, _lib.load().hattn_rotary, q.data_ptr(), _lib.ptr(k), _Strides(*strides),
+                qo.data_ptr(), _lib.ptr(ko), freqs.data_ptr(), freqs.dtype == torch.float64,
+                _lib.ptr(positions), wide, pb, pt, per_row, B, T, H, G, D, freqs.shape[0], interleaved,
+                scale, inverse, _lib.dtype_code(q))
     return qo, ko
 
 
@@ -152,23 +162,17 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Te
         raise NotImplementedError(f"D={D} above {MAX_D}")
     if not math.isfinite(scale) or abs(scale) > 1e30:
         raise ValueError(f"scale={scale}")
-    B = q.shape[0]
     if positions is not None:
-        if positions.shape not in ((B,), () if one else tuple(q.shape[:2])):
+        if positions.shape != q.shape[:1] and (one or positions.shape != q.shape[:2]):
             raise ValueError(f"positions {tuple(positions.shape)} for q {tuple(q.shape)}")
         if positions.dtype not in (torch.int32, torch.int64):
             raise NotImplementedError(f"positions in {positions.dtype}")
     elif one:
         raise ValueError("one token a row needs positions [B]")
     _lib.require_device(q, k, freqs, positions)
-    freqs = freqs.detach().contiguous()
-    if one:
-        q, k = q.unsqueeze(1), k.unsqueeze(1) if k is not None else None
+    if not freqs.is_contiguous():
+        freqs = freqs.contiguous()
     args = q, k, freqs, positions, layout == "interleaved", float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        q, k = RotaryFunction.apply(*args)
-    else:
-        q, k = _launch(*args, False)
-    if one:
-        q, k = q.squeeze(1), k.squeeze(1) if k is not None else None
-    return q, k
+        return RotaryFunction.apply(*args)
+    return _launch(*args, False)

@@ -181,7 +181,7 @@ def test_rotary_codes(kw, st):
     a.update(kw)
     p = 16 if st == NOT else None  # placeholders that no launch sees
     strides = (ctypes.c_longlong * 6)(0, 0, 0, 0, 0, 0)
-    assert code("hattn_rotary", p, p, strides, p, p, p, 1, None, 0, None, 0,
+    assert code("hattn_rotary", p, p, strides, p, p, p, 1, None, 0, 0, 0, 0,
                 *(a[n] for n in ("B", "T", "H", "G", "D", "pairs")), 0, a["scale"], 0, a["dtype"],
                 None) == st
 
@@ -240,9 +240,9 @@ def test_alignment_strides_and_workspace_codes():
                 2, 64, 128, 0, None) == VAL
     assert code("hattn_quant_cache_append", p, 72, None, s(64, 64, 64, 64, 64, 64), p, p, p, p, p, 1, 4,
                 2, 64, 128, 0, None) == VAL
-    assert code("hattn_rotary", 65, None, s(0, 0, 0, 0, 0, 0), p, None, p, 1, None, 0, None, 0, 1, 1, 1,
+    assert code("hattn_rotary", 65, None, s(0, 0, 0, 0, 0, 0), p, None, p, 1, None, 0, 0, 0, 0, 1, 1, 1,
                 0, 64, 32, 0, 1.0, 0, 0, None) == VAL
-    assert code("hattn_rotary", p, None, s(0, 0, 0, 0, 0, 0), p, None, 68, 1, None, 0, None, 0, 1, 1, 1,
+    assert code("hattn_rotary", p, None, s(0, 0, 0, 0, 0, 0), p, None, 68, 1, None, 0, 0, 0, 0, 1, 1, 1,
                 0, 64, 32, 0, 1.0, 0, 0, None) == VAL
 
 
