@@ -74,19 +74,24 @@ QuantArgs cache_args(const void* kc, const void* vc, const float* ks, const floa
 // Blocks that T tokens from any place on can touch.
 int touched(int T) { return (T + kQuantBlock - 2) / kQuantBlock + 1; }
 
-// How a call's queries are cut: blocks of 16 where a row and key head has at most kFewQueries,
-// else of 128; and parts of a row's tokens, enough that the card has work.
+// How a call's queries are cut: blocks of 16 or 32 where a row and key head has at most kFewQueries,
+// else of 128; and parts of a row's tokens, enough that the card has work.  With few rows a workgroup's
+// start counts, and 1024 of them (512 with two blocks of queries each) are best: 4 rows of 8000
+// to 32000 tokens, 8 key heads of 128: 43 us with 1024, 46 with 2048, 52 with 4096.  With many rows,
+// whose lengths differ, more even out the end: 64 rows of up to 9000 tokens 128, 126, 127 us.
 struct Cut {
   bool few;
   int rblocks, splits;
 };
-const int kFewQueries = 32;
+const int kFewQueries = 128;
 Cut cut(int B, int T, int H, int G, int capacity) {
   Cut c;
   const long queries = (long)T * (H / G);
   c.few = queries <= kFewQueries;
-  c.rblocks = (int)(c.few ? (queries + 15) / 16 : (queries + 127) / 128);
-  const long base = (long)B * G * c.rblocks, want = ((c.few ? 1024 : 512) + base - 1) / base;
+  c.rblocks = (int)(c.few ? (queries + 31) / 32 : (queries + 127) / 128);
+  const long base = (long)B * G * c.rblocks;
+  const long target = !c.few || queries > 16 ? 512 : base < 128 ? 1024 : 2048;
+  const long want = (target + base - 1) / base;
   const long most = (capacity + 255) / 256;
   c.splits = (int)std::max(1L, std::min({want, most, (long)kQuantSplits}));
   return c;
@@ -101,12 +106,18 @@ int attention_checks(int B, int T, int H, int G, int D, int capacity, float scal
   if ((double)T * (H / G) > (double)(INT_MAX / 2))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "T=%d H=%d: 2^30 queries of a key head or more", T, H);
   const Cut c = cut(B, T, H, G, capacity);
-  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) || !fits((double)B * T * H, 256))
+  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) || !fits((double)B * T * H, 512))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: 2^24 workgroups or more", B, T, H);
   return HATTN_OK;
 }
 
 bool joins(const Cut& c) { return c.few || c.splits > 1; }
+
+// Workspace in floats: the parts, their maxima and sums, and the rows' tokens during a step.
+size_t part_floats(int B, int T, int H, const Cut& c, int D) { return (size_t)B * T * H * c.splits * D; }
+size_t workspace_bytes(int B, int T, int H, const Cut& c, int D) {
+  return (part_floats(B, T, H, c, D) + (size_t)B * T * H * c.splits * 2 + B) * sizeof(float);
+}
 
 // The attention's launches on tensors that have been checked.
 int attend(QuantArgs& p, const void* q, const long long* strides, void* o, int T, int H, float scale,
@@ -119,7 +130,8 @@ int attend(QuantArgs& p, const void* q, const long long* strides, void* o, int T
   p.splits = c.splits; p.rblocks = c.rblocks;
   p.scale2 = scale * kLog2e;
   p.part = (float*)ws;
-  p.stat = p.part + (size_t)p.B * T * H * c.splits * p.D;
+  p.stat = p.part + part_floats(p.B, T, H, c, p.D);
+  p.held = (int*)(p.stat + (size_t)p.B * T * H * c.splits * 2);
   if (int st = check_hip(c.few ? hattn_quant_few_launch(p, dtype, stream)
                                : hattn_quant_chunk_launch(p, dtype, stream),
                          "attention over a cache launch"))
@@ -240,7 +252,7 @@ int hattn_quant_cache_read(const void* k_codes, const void* v_codes, const float
 size_t hattn_quant_cache_attention_workspace(int B, int T, int H, int G, int D, int capacity) {
   if (attention_checks(B, T, H, G, D, capacity, 1.f, HATTN_BF16)) return 0;
   const Cut c = cut(B, T, H, G, capacity);
-  return joins(c) ? (size_t)B * T * H * c.splits * (D + 2) * sizeof(float) : 0;
+  return joins(c) ? workspace_bytes(B, T, H, c, D) : 0;
 }
 
 int hattn_quant_cache_attention(const void* q, const int* lengths, const long long* strides,
@@ -277,9 +289,13 @@ int hattn_quant_cache_step(const void* q, const void* k, const void* v, const lo
   p.kb = strides[3]; p.kt = strides[4]; p.kh = strides[5];
   p.vb = strides[6]; p.vt = strides[7]; p.vh = strides[8];
   p.T = 1;
-  if (int st = check_hip(hattn_quant_token_launch(p, dtype, (hipStream_t)stream),
-                         "hattn_quant_cache_step launch"))
-    return st;
+  // Where one workgroup has all queries of a key head, it takes in the token too: a launch less
+  // (with 17 to 32 queries the kernel has no registers left for it)
+  p.coming = H / G <= 16;
+  if (!p.coming)
+    if (int st = check_hip(hattn_quant_token_launch(p, dtype, (hipStream_t)stream),
+                           "hattn_quant_cache_step launch"))
+      return st;
   return attend(p, q, strides, o, 1, H, scale, dtype, ws, ws_bytes, (hipStream_t)stream);
 }
 

@@ -16,9 +16,11 @@ struct QuantArgs {
   int* counts;                    // [B]: tokens that each row has had
   void *o, *ko, *vo;              // o [B, T, H, D]; read: ko, vo [B, n, G, D]
   float *part, *stat;             // [B, T, H, splits, D], [B, T, H, splits, 2]
+  int* held;                      // [B], where `coming`: tokens with the new one, or -1 where it has no slot
   int B, T, H, G, D, cap;
   int start, n;                   // read: slots [start, start + n)
   int blocks;                     // append, read: blocks of a row, at most
+  int coming;                     // one token a row enters the cache in the attention itself
   int splits, rblocks;            // attention: parts of a row's tokens, blocks of its queries
   float scale2;                   // scale * log2(e)
 };
@@ -28,7 +30,9 @@ hipError_t hattn_quant_append_launch(const QuantArgs& p, int dtype, hipStream_t 
 // One token a row; the counts advance in the same launch.
 hipError_t hattn_quant_token_launch(const QuantArgs& p, int dtype, hipStream_t stream);
 hipError_t hattn_quant_read_launch(const QuantArgs& p, int dtype, hipStream_t stream);
-// Blocks of 16 queries (few) or 128 (chunk) of a row and key head.
+// Blocks of 16 or 32 queries (few: 32 where there are more than 16) or 128 (chunk) of a row and key
+// head.  With `coming` (at most 16 queries)
+// the token enters the cache, and the join advances the counts.
 hipError_t hattn_quant_few_launch(const QuantArgs& p, int dtype, hipStream_t stream);
 hipError_t hattn_quant_chunk_launch(const QuantArgs& p, int dtype, hipStream_t stream);
 hipError_t hattn_quant_join_launch(const QuantArgs& p, int dtype, hipStream_t stream);

@@ -8,17 +8,6 @@
 
 namespace hattn {
 
-__device__ __forceinline__ unsigned wave_max(unsigned x) {
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) x = max(x, (unsigned)__shfl_xor((int)x, k, 64));
-  return x;
-}
-
-// The larger of the halves' finite magnitudes.
-template <typename E>
-__device__ __forceinline__ unsigned top2(unsigned x) {
-  return max(finite_bits<E>(x & 0xffff), finite_bits<E>(x >> 16));
-}
 template <typename E>
 __device__ __forceinline__ unsigned top8(uint4 x) {
   return max(max(top2<E>(x.x), top2<E>(x.y)), max(top2<E>(x.z), top2<E>(x.w)));
@@ -29,11 +18,12 @@ template <typename E, int PC>
 __global__ __launch_bounds__(256) void quant_append_kernel(QuantArgs p) {
   constexpr int ROWS = 256 >> PC, N = ROWS >= kQuantBlock ? 1 : kQuantBlock / ROWS;
   __shared__ unsigned tops[4];
-  long item = blockIdx.x;
+  unsigned item = blockIdx.x;  // 32-bit divisions: 64-bit ones are hundreds of instructions
   const bool isv = item & 1;
   item >>= 1;
-  const int j = item % p.blocks;
-  const int bg = (int)(item / p.blocks), b = bg / p.G, g = bg % p.G;
+  const int j = item % (unsigned)p.blocks;
+  const int bg = (int)(item / (unsigned)p.blocks);
+  const int b = (unsigned)bg / (unsigned)p.G, g = bg - b * p.G;
   const int n0 = max(p.counts[b], 0);
   const int fresh = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   const long first = ((long)(n0 / kQuantBlock) + j) * kQuantBlock;  // the block's first slot
@@ -90,41 +80,15 @@ __global__ __launch_bounds__(256) void quant_advance_kernel(QuantArgs p) {
   p.counts[b] = (int)min((long)max(p.counts[b], 0) + fresh, 0x7fffffffL);
 }
 
-// One token: a workgroup makes a row's codes of all heads, a wave one head of K or V at a time,
-// and then advances the row's count, which no other workgroup reads.
+// One token: a workgroup makes a row's codes of all heads, a wave one head at a time, and then
+// advances the row's count, which no other workgroup reads.
 template <typename E>
 __global__ __launch_bounds__(1024) void quant_token_kernel(QuantArgs p) {
-  const int b = blockIdx.x, lane = threadIdx.x & 63;
+  const int b = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int n0 = max(p.counts[b], 0);
-  if (n0 < p.cap) {
-    const int lo = n0 % kQuantBlock, first = n0 - lo;
-    for (int i = wave; i < 2 * p.G; i += waves) {
-      const bool isv = i & 1;
-      const int g = i >> 1;
-      const long bg = (long)b * p.G + g;
-      float* scale = (isv ? p.vs : p.ks) + bg * (p.cap / kQuantBlock) + first / kQuantBlock;
-      unsigned char* codes = (isv ? p.vc : p.kc) + (bg * p.cap + first) * p.D;
-      const __bf16* x = (const __bf16*)(isv ? p.v : p.k) + b * (isv ? p.vb : p.kb) +
-                        g * (isv ? p.vh : p.kh);
-      const float was = lo > 0 ? *scale : 0.f;
-      const bool mine = 2 * lane < p.D;
-      const unsigned y = mine ? *(const unsigned*)(x + 2 * lane) : 0;
-      const float now = fmaxf(power(scale_exponent<E>(wave_max(top2<E>(y)))), was);
-      const int c = codes2<E, false>(y, 1.f / now, 0);
-      if (mine) *(unsigned short*)(codes + lo * p.D + 2 * lane) = (unsigned short)c;
-      if (lane == 0) *scale = now;
-      if (lo > 0 && now > was) {
-        const float ratio = was / now;
-        for (int at = 16 * lane; at < lo * p.D; at += 1024) {
-          uint4 old = *(const uint4*)(codes + at);
-          old = uint4{rescale4(old.x, ratio), rescale4(old.y, ratio), rescale4(old.z, ratio),
-                      rescale4(old.w, ratio)};
-          *(uint4*)(codes + at) = old;
-        }
-      }
-    }
-  }
+  if (n0 < p.cap)
+    for (int i = wave; i < p.G; i += waves) token_codes<E>(p, b, i, n0);
   __syncthreads();
   if (threadIdx.x == 0) p.counts[b] = min(n0, 0x7ffffffe) + 1;
 }
@@ -134,11 +98,12 @@ __global__ __launch_bounds__(1024) void quant_token_kernel(QuantArgs p) {
 template <typename T, int PC>
 __global__ __launch_bounds__(256) void quant_read_kernel(QuantArgs p) {
   constexpr int ROWS = 256 >> PC, N = ROWS >= kQuantBlock ? 1 : kQuantBlock / ROWS;
-  long item = blockIdx.x;
+  unsigned item = blockIdx.x;  // 32-bit divisions: 64-bit ones are hundreds of instructions
   const bool isv = item & 1;
   item >>= 1;
-  const int j = item % p.blocks;
-  const int bg = (int)(item / p.blocks), b = bg / p.G, g = bg % p.G;
+  const int j = item % (unsigned)p.blocks;
+  const int bg = (int)(item / (unsigned)p.blocks);
+  const int b = (unsigned)bg / (unsigned)p.G, g = bg - b * p.G;
   const int first = (p.start / kQuantBlock + j) * kQuantBlock;
   const int count = p.counts[b], end = p.start + p.n;
   const float scale = (isv ? p.vs : p.ks)[(long)bg * (p.cap / kQuantBlock) + first / kQuantBlock];
@@ -201,7 +166,7 @@ hipError_t hattn_quant_append_launch(const QuantArgs& p, int dtype, hipStream_t 
 
 hipError_t hattn_quant_token_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
   using namespace hattn;
-  const dim3 grid((unsigned)p.B), block(64 * (2 * p.G < 16 ? 2 * p.G : 16));
+  const dim3 grid((unsigned)p.B), block(64 * (p.G < 16 ? p.G : 16));
   if (dtype == 1)
     hipLaunchKernelGGL((quant_token_kernel<_Float16>), grid, block, 0, stream, p);
   else

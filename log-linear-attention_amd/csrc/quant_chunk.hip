@@ -7,9 +7,10 @@
 //   S^T = K Q^T,  P = exp2(c ks S - m),  O^T += vs V^T P^T,  c = scale log2(e)
 // on the codes.  Codes are exact in 16 bits: the workgroup widens each tile once, between the
 // registers that its bytes come to, one tile ahead, and LDS, in the layout of sliding_device.h.
-// A tile has one scale of K, which multiplies its scores.  Its scale of V is folded into P's
-// exponent in bf16, whose range holds it; in fp16, whose range does not, it multiplies the tile's part
-// of the sum.
+// A block of 64 slots has one scale of K, which multiplies its scores, and one of V, which is folded into
+// P's exponent.  In bf16 its range holds that.  In fp16 the sums are in units of a scale near
+// the block's own (at least 2^-40: smaller values are 0 in the result), so that P is folded by
+// at most 2^-8, which its lift makes up for.
 //
 // Where blocks are few, a row's slots are cut over workgroups too, whose partial results
 // quant_few.hip's second kernel joins.
@@ -18,30 +19,43 @@
 
 namespace hattn {
 
+// x of lanes ln and ln + 32, in both; x comes from a vector instruction, not from a matrix product.
+struct Halves {
+  float lo, hi;
+  __device__ __forceinline__ explicit Halves(float x) {
+    lo = hi = x;
+    // as assembly: the compiler takes the builtin's two results for one.  The instruction reads
+    // what vector instructions wrote two states ago at the latest.
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi));
+  }
+};
+
+constexpr float kLeastUnit = 0x1p-40f;
+
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(QuantArgs p) {
-  constexpr int BN = 32;
-  constexpr bool FOLD = !__is_same(E, _Float16);
+  constexpr int BN = kQuantBlock, N = BN * DP / 2048;  // 16-byte pieces of K and V that a thread widens
+  constexpr bool UNITS = __is_same(E, _Float16);
+  // apart, not indexed, so that the compiler sees which of them is written
   __shared__ __attribute__((aligned(16))) __bf16 K0[BN * DP], K1[BN * DP], V0[BN * DP], V1[BN * DP];
   const int lane = threadIdx.x & 63, ln = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = p.H / p.G;
-  const long item = work_item((long)p.B * p.G * p.rblocks * p.splits);
-  if (item < 0) return;
-  const int split = item % p.splits;
+  const long place = work_item((long)p.B * p.G * p.rblocks * p.splits);
+  if (place < 0) return;
+  const unsigned item = (unsigned)place;  // below 2^24
+  const int split = item % (unsigned)p.splits;
   // the last queries, which see the most, first
-  const int blk = p.rblocks - 1 - (int)(item / p.splits % p.rblocks);
-  const int bg = (int)(item / p.splits / p.rblocks), b = bg / p.G, g = bg % p.G;
+  const int blk = p.rblocks - 1 - (int)(item / (unsigned)p.splits % (unsigned)p.rblocks);
+  const int bg = (int)(item / (unsigned)p.splits / (unsigned)p.rblocks), b = bg / p.G, g = bg % p.G;
   const QuantRow row(p, b);
   const int each = part_tokens(row.n, p.splits);
   const int from = (int)min((long)split * each, (long)row.n);
   const int q0 = blk * 128, qw = q0 + 32 * wave, query = qw + ln;
   const int t = query / R, r = query - t * R, end = row.end(t);
-  // what the block, and the wave, see at most, and what each of the wave's queries sees; blocks
-  // and waves of padding see nothing
+  // what the block, and the wave, see at most; blocks and waves of padding see nothing
   const int to = q0 / R < row.fresh ? min(from + each, row.end(min((q0 + 127) / R, row.fresh - 1))) : 0;
   const int most = qw / R < row.fresh ? row.end(min((qw + 31) / R, row.fresh - 1)) : 0;
-  const int least = row.end(qw / R);
   const bool mine = t < p.T;
   const long at = ((long)b * p.T + t) * p.H + g * R + r;
 
@@ -49,6 +63,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = zero16();
   float m = -3e38f, l = 0.f;  // below every score; not -inf, whose difference is NaN
+  float vunit = 1.f;          // what acc is in units of
 
   if (from < to) {
     const unsigned char* kc = p.kc + (long)bg * p.cap * p.D;
@@ -59,87 +74,121 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
     load_frags<DP>((const __bf16*)p.q + b * p.qb + min(t, row.fresh - 1) * p.qt +
                        (g * R + (t < row.fresh ? r : 0)) * p.qh, p.D, qf);
 
-    // 16 bytes of one slot's K or V: with D 128 both from every thread, else one
-    constexpr int PIECES = DP / 16, N = DP / 64;
-    const int rw = threadIdx.x / PIECES % BN, pc = threadIdx.x % PIECES;
+    // pieces pc of slots rw, rw + 4096 / DP, .. of a block: first K's, then V's
+    constexpr int PIECES = DP / 16, ROWS = 256 / PIECES;
+    const int rw = threadIdx.x / PIECES, pc = threadIdx.x % PIECES;
     uint4 raw[N];
+    float kscale = ks[from / kQuantBlock], vscale = vs[from / kQuantBlock], knext, vnext;
+    if (UNITS) vunit = fmaxf(vscale, kLeastUnit);
+    // slots past the end read the last one, and pieces past D the row's first: Q is zero there, or the
+    // result is not stored
     const auto fetch = [&](int s0) __attribute__((always_inline)) {
-      const long o = (long)min(s0 + rw, to - 1) * p.D + 16 * pc;
+      knext = ks[s0 / kQuantBlock];
+      vnext = vs[s0 / kQuantBlock];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bool isv = N == 2 ? i == 1 : threadIdx.x >= BN * PIECES;
-        raw[i] = 16 * pc < p.D ? *(const uint4*)((isv ? vc : kc) + o) : uint4{};
+        const long o = (long)min(s0 + rw + i % (N / 2) * ROWS, to - 1) * p.D;
+        raw[i] = *(const uint4*)((i < N / 2 ? kc : vc) + o + (16 * pc < p.D ? 16 * pc : 0));
       }
     };
     const auto put = [&](__bf16* K, __bf16* V) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const bool isv = N == 2 ? i == 1 : threadIdx.x >= BN * PIECES;
-        __bf16* X = (isv ? V : K) + rw * DP;
-        *(bf16x8*)(X + ((2 * pc) ^ swizzle<DP>(rw)) * 8) = widen8<E>(raw[i].x, raw[i].y);
-        *(bf16x8*)(X + ((2 * pc + 1) ^ swizzle<DP>(rw)) * 8) = widen8<E>(raw[i].z, raw[i].w);
+        const int r = rw + i % (N / 2) * ROWS;
+        __bf16* X = (i < N / 2 ? K : V) + r * DP;
+        *(bf16x8*)(X + ((2 * pc) ^ swizzle<DP>(r)) * 8) = widen8<E>(raw[i].x, raw[i].y);
+        *(bf16x8*)(X + ((2 * pc + 1) ^ swizzle<DP>(r)) * 8) = widen8<E>(raw[i].z, raw[i].w);
       }
+      kscale = knext;
+      vscale = vnext;
     };
     const auto part = [&](auto MASK, int s0, const __bf16* K, const __bf16* V)
                           __attribute__((always_inline)) {
-      const float kscale = ks[s0 / kQuantBlock] * p.scale2, vscale = vs[s0 / kQuantBlock];
-      floatx16 s = zero16();
+      const float unit = kscale * p.scale2;
+      floatx16 s[2];
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) s = mfma32<E>(row_frag<DP>(K, 0, c), qf[c], s);
-      if constexpr (MASK.value) {
-        const int up = end - s0 - 4 * hf;
+      for (int h = 0; h < 2; ++h) {
+        bf16x8 kf[DP / 16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < up ? s[i] : -INFINITY;
+        for (int c = 0; c < DP / 16; ++c) kf[c] = row_frag<DP>(K, 32 * h, c);
+        __builtin_amdgcn_sched_barrier(0);
+        s[h] = zero16();
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) s[h] = mfma32<E>(kf[c], qf[c], s[h]);
       }
-      float top = fmaxf(s[0], s[1]);
+      if constexpr (MASK.value) {
 #pragma unroll
-      for (int i = 2; i < 16; i += 2) top = max3(top, s[i], s[i + 1]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * kscale;
-      if (__any(top > m + 8.f)) {
+        for (int h = 0; h < 2; ++h) {
+          const int up = end - s0 - 32 * h - 4 * hf;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][i] = 8 * (i >> 2) + (i & 3) < up ? s[h][i] : -INFINITY;
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      float top = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2) top = max3(top, s[0][i], s[0][i + 1]);
+      float top1 = fmaxf(s[1][0], s[1][1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2) top1 = max3(top1, s[1][i], s[1][i + 1]);
+      const Halves both(fmaxf(top, top1));
+      top = fmaxf(both.lo, both.hi) * unit;
+      if (__any(top > m + Half<E>::kSlack)) {
         const float m2 = fmaxf(m, top), shrink = exp2_(m - m2);
         m = m2;
         l *= shrink;
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= shrink;
       }
-      const float base = FOLD ? m - log2f(vscale) : m;
+      if (UNITS && __any(vscale > vunit || (vscale < vunit * 0x1p-8f && vunit > kLeastUnit))) {
+        const float next = fmaxf(vscale, kLeastUnit);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= vunit / next;
+        vunit = next;
+      }
+      const float ratio = UNITS ? vscale * __builtin_amdgcn_rcpf(vunit) : vscale;
+      const float base = m - Half<E>::kLift - __builtin_amdgcn_logf(ratio);
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] = exp2_(fmaf(s[i], kscale, -base));
-        sum += s[i];
-      }
-      l += FOLD ? sum / vscale : sum;
-      const bf16x8 pf[2] = {pack8<E>(s, 0), pack8<E>(s, 1)};
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
-        floatx16 o = FOLD ? acc[dt] : zero16();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) o = mfma32<E>(tr32<DP>(V, 16 * c, 32 * dt), pf[c], o);
-        if constexpr (FOLD) {
-          acc[dt] = o;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[dt][i] = fmaf(o[i], vscale, acc[dt][i]);
+        for (int i = 0; i < 16; ++i) {
+          s[h][i] = exp2_(fmaf(s[h][i], unit, -base));
+          sum += s[h][i];
         }
       }
+      l = fmaf(sum, __builtin_amdgcn_rcpf(ratio), l);
+      __builtin_amdgcn_s_setprio(1);
+      const bf16x8 pf[4] = {pack8<E>(s[0], 0), pack8<E>(s[0], 1), pack8<E>(s[1], 0), pack8<E>(s[1], 1)};
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          acc[dt] = mfma32<E>(tr32<DP>(V, 16 * c, 32 * dt), pf[c], acc[dt]);
+      __builtin_amdgcn_s_setprio(0);
     };
-    const auto step = [&](int s0, const __bf16* K, const __bf16* V, __bf16* Kn, __bf16* Vn)
+    const auto step = [&](auto MASK, int s0, const __bf16* K, const __bf16* V, __bf16* Kn, __bf16* Vn)
                           __attribute__((always_inline)) {
       __syncthreads();
       const bool more = s0 + BN < to;
       if (more) fetch(s0 + BN);
-      if (s0 + BN <= least) part(Bool<false>(), s0, K, V);
-      else if (s0 < most) part(Bool<true>(), s0, K, V);
+      if (!MASK.value || s0 < most) part(MASK, s0, K, V);
       if (more) put(Kn, Vn);
     };
     fetch(from);
     put(K0, V0);
-    for (int s0 = from; s0 < to; s0 += 2 * BN) {
-      step(s0, K0, V0, K1, V1);
-      if (s0 + BN < to) step(s0 + BN, K1, V1, K0, V0);
-    }
-    l += __shfl_xor(l, 32, 64);
+    int s0 = from;
+    const auto pair = [&](auto MASK) __attribute__((always_inline)) {
+      step(MASK, s0, K0, V0, K1, V1);
+      if (!MASK.value || s0 + BN < to) step(MASK, s0 + BN, K1, V1, K0, V0);
+    };
+    // blocks that all queries see whole, in pairs, then those that need masks
+    for (const int whole = min(row.end(q0 / R), to); s0 + 2 * BN <= whole; s0 += 2 * BN)
+      pair(Bool<false>());
+    for (; s0 < to; s0 += 2 * BN) pair(Bool<true>());
+    const Halves both(l);
+    l = both.lo + both.hi;
   }
 
   if (p.splits == 1) {
@@ -152,7 +201,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
         for (int i = 0; i < 16; ++i) acc[dt][i] = __builtin_nanf("");
       store_t<E, DP>(o, acc, 1.f, true, p.D);
     } else {
-      store_t<E, DP>(o, acc, 1.f / l, end > 0, p.D);
+      store_t<E, DP>(o, acc, vunit / l, end > 0, p.D);
     }
     return;
   }
@@ -166,7 +215,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
       const int d = 32 * dt + 8 * i + 4 * hf;
       floatx4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * i + j];
+      for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * i + j] * vunit;
       if (d < p.D) *(floatx4*)(p.part + to_part * p.D + d) = x;
     }
   if (hf == 0) {

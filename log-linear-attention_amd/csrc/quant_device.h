@@ -23,12 +23,19 @@ template <>
 struct Half<__bf16> {
   static constexpr unsigned kInf = 0x7f80;
   static constexpr int kMost = 119;
+  static constexpr float kSlack = 8.f, kLift = 0.f;
 };
 template <>
 struct Half<_Float16> {
   static constexpr unsigned kInf = 0x7c00;
   static constexpr int kMost = 7;
+  static constexpr float kSlack = 4.f, kLift = 11.f;
 };
+
+// The running maximum m of a query's scores (powers of two) is taken again only where a score passes
+// it by more than kSlack, so that most tiles do not rescale the sums; probabilities are
+// 2^(s - m + kLift), at most 2^15.  In fp16 the lift keeps those down to 2^-25 of the largest out of
+// the subnormal numbers: of many tokens of little weight each, the sum would be off.
 
 // The magnitude of a 16-bit number as an integer of the same order; 0 where it is not finite.
 template <typename E>
@@ -98,17 +105,68 @@ __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi) {
   return bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) x = max(x, (unsigned)__shfl_xor((int)x, k, 64));
+  return x;
+}
+
+// The larger of the halves' finite magnitudes.
+template <typename E>
+__device__ __forceinline__ unsigned top2(unsigned x) {
+  return max(finite_bits<E>(x & 0xffff), finite_bits<E>(x >> 16));
+}
+// One new token of row b and key head g enters slot n0, by one wave: its codes, the block's scales,
+// and where these grow the block's older codes.
+template <typename E>
+__device__ __forceinline__ void token_codes(const QuantArgs& p, int b, int g, int n0) {
+  const int lane = threadIdx.x & 63, lo = n0 % kQuantBlock, first = n0 - lo;
+  const long bg = (long)b * p.G + g, block = bg * (p.cap / kQuantBlock) + first / kQuantBlock;
+  const bool mine = 2 * lane < p.D;
+  float* const scale[2] = {p.ks + block, p.vs + block};
+  unsigned char* const codes[2] = {p.kc + (bg * p.cap + first) * p.D, p.vc + (bg * p.cap + first) * p.D};
+  const __bf16* const x[2] = {(const __bf16*)p.k + b * p.kb + g * p.kh,
+                              (const __bf16*)p.v + b * p.vb + g * p.vh};
+  unsigned y[2], top[2];
+  float was[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    y[i] = mine ? *(const unsigned*)(x[i] + 2 * lane) : 0;
+    was[i] = lo > 0 ? *scale[i] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) top[i] = wave_max(top2<E>(y[i]));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float now = fmaxf(power(scale_exponent<E>(top[i])), was[i]);
+    const int c = codes2<E, false>(y[i], 1.f / now, 0);
+    if (mine) *(unsigned short*)(codes[i] + lo * p.D + 2 * lane) = (unsigned short)c;
+    if (lane == 0) *scale[i] = now;
+    if (lo > 0 && now > was[i]) {
+      const float ratio = was[i] / now;
+      for (int at = 16 * lane; at < lo * p.D; at += 1024) {
+        uint4 old = *(const uint4*)(codes[i] + at);
+        old = uint4{rescale4(old.x, ratio), rescale4(old.y, ratio), rescale4(old.z, ratio),
+                    rescale4(old.w, ratio)};
+        *(uint4*)(codes[i] + at) = old;
+      }
+    }
+  }
+}
+
 // What a row has: tokens in its cache (none where the count has passed the capacity: `full`), and
-// its new tokens.
+// its new tokens.  `coming`: its one new token is not counted yet.
 struct QuantRow {
   int n, fresh;
   bool full;
-  __device__ __forceinline__ QuantRow(const QuantArgs& p, int b) {
+  __device__ __forceinline__ QuantRow(const QuantArgs& p, int b, bool coming = false) {
     const int c = max(p.counts[b], 0);
-    full = c > p.cap;
-    n = full ? 0 : c;
+    full = c > p.cap - coming;
+    n = full ? 0 : c + coming;
     fresh = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
   }
+  // One new token, from what the attention's kernel noted.
+  __device__ __forceinline__ explicit QuantRow(int held) : n(max(held, 0)), fresh(1), full(held < 0) {}
   // The slots that query t of the new ones sees end before this.
   __device__ __forceinline__ int end(int t) const {
     return t < fresh ? max(n - fresh + t + 1, 0) : 0;

@@ -1,7 +1,7 @@
 // Attention of a few queries over a cache in 8 bits: one token a row, or some drafted ones.
 //
 // The queries of a row that share a key head, query t of head r as t * R + r, are the columns of
-// 16x16x32 products, 16 to a workgroup:
+// 16x16x32 products, 16 or 32 to a workgroup:
 //   S^T[slot][query] = K Q^T,  P = exp2(c ks S - m),  O^T[d][query] += vs V^T P^T
 // on the codes themselves, which are exact in 16 bits: the scale ks of a block of keys multiplies
 // its scores, and vs the block's part of the sum.  P is rounded to the inputs' type.
@@ -28,36 +28,51 @@ __device__ __forceinline__ void transpose4(const unsigned (&a)[4], unsigned (&t)
   t[3] = __builtin_amdgcn_perm(y1, x1, 0x07060302);
 }
 
-template <typename E, int DP>
+template <typename E, int DP, int NB, bool COMING>
 __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
   constexpr int W = DP / 64;   // words of a slot's V that a lane holds; 16-byte pieces of its K
   __shared__ __attribute__((aligned(16))) float part[4 * 16 * DP];
-  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float sm[4][16 * NB], sl[4][16 * NB];
   const int lane = threadIdx.x & 63, ln = lane & 15, lq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int R = p.H / p.G;
-  long item = blockIdx.x;
-  const int split = item % p.splits;
-  item /= p.splits;
-  const int rb = item % p.rblocks, bg = (int)(item / p.rblocks), b = bg / p.G, g = bg % p.G;
-  const QuantRow row(p, b);
+  unsigned item = blockIdx.x;  // 32-bit divisions: 64-bit ones are hundreds of instructions
+  const int split = item % (unsigned)p.splits;
+  item /= (unsigned)p.splits;
+  const int rb = item % (unsigned)p.rblocks, bg = (int)(item / (unsigned)p.rblocks);
+  const int b = (unsigned)bg / (unsigned)p.G, g = bg - b * p.G;
+  const QuantRow row(p, b, COMING);
+  // for the join, which advances the counts
+  if (COMING && split == 0 && g == 0 && threadIdx.x == 0) p.held[b] = row.full ? -1 : row.n;
   const int each = part_tokens(row.n, p.splits);
   const int from = (int)min((long)split * each, (long)row.n), to = min(from + each, row.n);
-  const int col = rb * 16 + ln, t = col / R, r = col - t * R;  // this lane's query
-  const int end = row.end(t), least = row.end(rb * 16 / R);    // the block's first sees least
-  if (from >= to) return;                                      // nor does the join read it
-
-  bf16x8 qf[W][2];
-#pragma unroll
-  for (int s = 0; s < W; ++s)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int d = 64 * s + 16 * lq + 8 * h;
-      qf[s][h] = t < row.fresh && d < p.D
-                     ? *(const bf16x8*)((const __bf16*)p.q + b * p.qb + t * p.qt +
-                                        (g * R + r) * p.qh + d)
-                     : bf16x8{};
+  if (from >= to) return;  // nor does the join read it
+  if constexpr (COMING) {
+    // by the wave that walks the new token's block, which no other reads
+    if (to == row.n && ((to - 1 - from) / kQuantBlock & 3) == wave) {
+      token_codes<E>(p, b, g, row.n - 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+  }
+  const int first = rb * 16 * NB, least = row.end((unsigned)first / (unsigned)R);  // the first query sees least
+
+  int end[NB];
+  bf16x8 qf[NB][W][2];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int query = first + 16 * nb + ln, t = (unsigned)query / (unsigned)R, r = query - t * R;
+    end[nb] = row.end(t);
+#pragma unroll
+    for (int s = 0; s < W; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 64 * s + 16 * lq + 8 * h;
+        qf[nb][s][h] = t < row.fresh && d < p.D
+                           ? *(const bf16x8*)((const __bf16*)p.q + b * p.qb + t * p.qt +
+                                              (g * R + r) * p.qh + d)
+                           : bf16x8{};
+      }
+  }
   const unsigned char* kc = p.kc + (long)bg * p.cap * p.D;
   const unsigned char* vc = p.vc + (long)bg * p.cap * p.D;
   const float* ks = p.ks + (long)bg * (p.cap / kQuantBlock);
@@ -65,20 +80,24 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
 
   uint4 K[4][W];
   unsigned V[2][2][4][W];
-  // slots past the end read the last one
+  float kscale, vscale;
+  // Slots past the end read the last one, and pieces past D the row's first (Q is zero there, or
+  // the result is not stored).
   const auto load_k = [&](int s0) __attribute__((always_inline)) {
+    kscale = ks[s0 / kQuantBlock];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
       const unsigned char* at = kc + (long)min(s0 + 16 * kt + ln, to - 1) * p.D;
 #pragma unroll
       for (int s = 0; s < W; ++s) {
         const int d = 64 * s + 16 * lq;
-        K[kt][s] = d < p.D ? *(const uint4*)(at + d) : uint4{};
+        K[kt][s] = *(const uint4*)(at + (d < p.D ? d : 0));
       }
     }
   };
   const auto load_v = [&](int s0) __attribute__((always_inline)) {
     const int d = 4 * W * ln;
+    vscale = vs[s0 / kQuantBlock];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -97,59 +116,76 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
         }
   };
 
-  float m = -3e38f, l = 0.f;  // below every score; not -inf, whose difference is NaN
-  floatx4 acc[DP / 16];       // element d = 4 W (4 lq + i) + n of acc[n][i]
+  float m[NB], l[NB];
+  floatx4 acc[NB][DP / 16];  // element d = 4 W (4 lq + i) + n of acc[..][n][i]
 #pragma unroll
-  for (int n = 0; n < DP / 16; ++n) acc[n] = zero4();
+  for (int nb = 0; nb < NB; ++nb) {
+    m[nb] = -3e38f;  // below every score; not -inf, whose difference is NaN
+    l[nb] = 0.f;
+#pragma unroll
+    for (int n = 0; n < DP / 16; ++n) acc[nb][n] = zero4();
+  }
   int s0 = from + kQuantBlock * wave;
   if (s0 < to) {
     load_k(s0);
     load_v(s0);
   }
   for (; s0 < to; s0 += 4 * kQuantBlock) {
-    const float kscale = ks[s0 / kQuantBlock] * p.scale2, vscale = vs[s0 / kQuantBlock];
-    floatx4 s[4];
+    const float unit = kscale * p.scale2;
+    floatx4 s[NB][4];
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-      s[kt] = zero4();
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[nb][kt] = zero4();
 #pragma unroll
       for (int c = 0; c < W; ++c) {
         const uint4 x = K[kt][c];
-        s[kt] = mfma16<E>(widen8<E>(x.x, x.y), qf[c][0], s[kt]);
-        s[kt] = mfma16<E>(widen8<E>(x.z, x.w), qf[c][1], s[kt]);
+        const bf16x8 lo = widen8<E>(x.x, x.y), hi = widen8<E>(x.z, x.w);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          s[nb][kt] = mfma16<E>(lo, qf[nb][c][0], s[nb][kt]);
+          s[nb][kt] = mfma16<E>(hi, qf[nb][c][1], s[nb][kt]);
+        }
       }
     }
     if (s0 + 4 * kQuantBlock < to) load_k(s0 + 4 * kQuantBlock);
     const bool whole = s0 + kQuantBlock <= min(least, to);  // every query sees the block whole
-    float top = -INFINITY;
+    bf16x8 pf[NB][2];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int nb = 0; nb < NB; ++nb) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[kt][i] *= kscale;
-        if (!whole) s[kt][i] = s0 + 16 * kt + 4 * lq + i < end ? s[kt][i] : -INFINITY;
-        top = fmaxf(top, s[kt][i]);
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = s[nb][kt][i] * unit;
+          if (!whole) x = s0 + 16 * kt + 4 * lq + i < end[nb] ? x : -INFINITY;
+          s[nb][kt][i] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m[nb] + Half<E>::kSlack)) {
+        const float m2 = fmaxf(m[nb], top), shrink = __builtin_amdgcn_exp2f(m[nb] - m2);
+        m[nb] = m2;
+        l[nb] *= shrink;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) acc[nb][n] *= shrink;
       }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m + 8.f)) {
-      const float m2 = fmaxf(m, top), shrink = __builtin_amdgcn_exp2f(m - m2);
-      m = m2;
-      l *= shrink;
+      const float base = m[nb] - Half<E>::kLift;
 #pragma unroll
-      for (int n = 0; n < DP / 16; ++n) acc[n] *= shrink;
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[nb][kt][i] = __builtin_amdgcn_exp2f(s[nb][kt][i] - base);
+          l[nb] += s[nb][kt][i];
+        }
+      pf[nb][0] = cat8e<E>(s[nb][0], s[nb][1]);
+      pf[nb][1] = cat8e<E>(s[nb][2], s[nb][3]);
     }
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[kt][i] = __builtin_amdgcn_exp2f(s[kt][i] - m);
-        l += s[kt][i];
-      }
-    const bf16x8 pf[2] = {cat8e<E>(s[0], s[1]), cat8e<E>(s[2], s[3])};
-#pragma unroll
     for (int w = 0; w < W; ++w) {
-      floatx4 o[4];
+      floatx4 o[NB][4];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         unsigned lo[4], hi[4], a[4], z[4];
@@ -161,74 +197,94 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
         transpose4(a, lo);
         transpose4(z, hi);
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-          o[n] = mfma16<E>(widen8<E>(lo[n], hi[n]), pf[c], c ? o[n] : zero4());
+        for (int n = 0; n < 4; ++n) {
+          const bf16x8 x = widen8<E>(lo[n], hi[n]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            o[nb][n] = mfma16<E>(x, pf[nb][c], c ? o[nb][n] : zero4());
+        }
       }
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[4 * w + n][i] = fmaf(o[n][i], vscale, acc[4 * w + n][i]);
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[nb][4 * w + n][i] = fmaf(o[nb][n][i], vscale, acc[nb][4 * w + n][i]);
     }
     if (s0 + 4 * kQuantBlock < to) load_v(s0 + 4 * kQuantBlock);
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
 
-  // the four waves' results; 4-element piece c of a query lies at c ^ query
-  float* mine = part + wave * 16 * DP + ln * DP;
+  // the four waves' results, 16 queries at a time; 4-element piece c of a query lies at c ^ query
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int nb = 0; nb < NB; ++nb) {
+    l[nb] += __shfl_xor(l[nb], 16, 64);
+    l[nb] += __shfl_xor(l[nb], 32, 64);
+    const int queries = p.T * R - first - 16 * nb;  // the others hold nothing
+    if (nb > 0) __syncthreads();
+    if (ln < queries) {
+      float* mine = part + wave * 16 * DP + ln * DP;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const int piece = W * (4 * lq + i) + w;
-      floatx4 x;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) x[n] = acc[4 * w + n][i];
-      *(floatx4*)(mine + (piece ^ ln) * 4) = x;
+        for (int w = 0; w < W; ++w) {
+          const int piece = W * (4 * lq + i) + w;
+          floatx4 x;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) x[n] = acc[nb][4 * w + n][i];
+          *(floatx4*)(mine + (piece ^ ln) * 4) = x;
+        }
+      if (lq == 0) {
+        sm[wave][16 * nb + ln] = m[nb];
+        sl[wave][16 * nb + ln] = l[nb];
+      }
     }
-  if (lq == 0) {
-    sm[wave][ln] = m;
-    sl[wave][ln] = l;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * DP / 4; i += 256) {
-    const int c = i / (DP / 4), d4 = i % (DP / 4), query = rb * 16 + c, tq = query / R;
-    if (tq >= p.T || 4 * d4 >= p.D) continue;
-    float top = sm[0][c];
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(queries, 16) * (DP / 4); i += 256) {
+      const int c = i / (DP / 4), d4 = i % (DP / 4), at = 16 * nb + c;
+      if (4 * d4 >= p.D) continue;
+      float top = sm[0][at];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w][c]);
-    floatx4 o = zero4();
-    float sum = 0.f;
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w][at]);
+      floatx4 o = zero4();
+      float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sm[w][c] - top);
-      const floatx4 x = *(const floatx4*)(part + (w * 16 + c) * DP + (d4 ^ c) * 4);
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sm[w][at] - top);
+        const floatx4 x = *(const floatx4*)(part + (w * 16 + c) * DP + (d4 ^ c) * 4);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = fmaf(x[k], f, o[k]);
-      sum += sl[w][c] * f;
-    }
-    const long at = ((((long)b * p.T + tq) * p.H + g * R + query - tq * R)) * p.splits + split;
-    *(floatx4*)(p.part + at * p.D + 4 * d4) = o;
-    if (d4 == 0) {
-      p.stat[2 * at] = top;
-      p.stat[2 * at + 1] = sum;
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(x[k], f, o[k]);
+        sum += sl[w][at] * f;
+      }
+      const unsigned query = first + at, t = query / (unsigned)R;
+      const long to_part =
+          ((((long)b * p.T + t) * p.H + g * R + query - t * R)) * p.splits + split;
+      *(floatx4*)(p.part + to_part * p.D + 4 * d4) = o;
+      if (d4 == 0) {
+        p.stat[2 * to_part] = top;
+        p.stat[2 * to_part + 1] = sum;
+      }
     }
   }
 }
 
-// Joins a query's partial results, those of the parts that have tokens: groups of lanes that hold
+// Joins a query's partial results, those of the parts that have tokens, and counts a step's new
+// tokens (no other workgroup reads the counts then): groups of lanes that hold
 // 4 elements each take every n-th part, and the groups' sums meet in LDS, in order.
 template <typename E>
 __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
   __shared__ float share[kQuantSplits];
   __shared__ floatx4 sums[256];
-  const long query = blockIdx.x, bt = query / p.H;
-  const int b = (int)(bt / p.T), t = (int)(bt - (long)b * p.T), lane = threadIdx.x & 63;
-  const QuantRow row(p, b);
+  const unsigned bt = blockIdx.x / (unsigned)p.H;
+  const long query = blockIdx.x;
+  const int b = (int)(bt / (unsigned)p.T), t = (int)(bt - (unsigned)b * p.T), lane = threadIdx.x & 63;
+  const QuantRow row = p.coming ? QuantRow(p.held[b]) : QuantRow(p, b);
+  if (p.coming && blockIdx.x == bt * p.H && blockIdx.y == 0 && threadIdx.x == 0)
+    p.counts[b] = min(max(p.counts[b], 0), 0x7ffffffe) + 1;
   __bf16* o = (__bf16*)p.o + query * p.D;
   if (row.end(t) == 0) {  // it sees nothing
     const float none = row.full && t < row.fresh ? __builtin_nanf("") : 0.f;
-    if (threadIdx.x < p.D) o[threadIdx.x] = to16<E>(none);
+    if (threadIdx.x < p.D && blockIdx.y == 0) o[threadIdx.x] = to16<E>(none);
     return;
   }
   const int each = part_tokens(row.n, p.splits), live = (row.n + each - 1) / each;
@@ -246,11 +302,12 @@ __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k, 64);
   __syncthreads();
-  const int pieces = p.D / 4, groups = 256 / pieces;
-  const int group = threadIdx.x / pieces, c = threadIdx.x - group * pieces;
+  // up to 64 elements a workgroup
+  const int c0 = blockIdx.y * 16, pieces = min(p.D / 4 - c0, 16), groups = 256 / pieces;
+  const int group = threadIdx.x / (unsigned)pieces, c = threadIdx.x - group * pieces;
   floatx4 x = zero4();
   if (group < groups) {
-    const float* part = p.part + query * p.splits * p.D + 4 * c;
+    const float* part = p.part + query * p.splits * p.D + 4 * (c0 + c);
 #pragma unroll 4
     for (int s = group; s < live; s += groups) {
       const floatx4 y = *(const floatx4*)(part + (long)s * p.D);
@@ -265,7 +322,7 @@ __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
   bf16x4 y;
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = to16<E>(x[i] / sum);
-  *(bf16x4*)(o + 4 * c) = y;
+  *(bf16x4*)(o + 4 * (c0 + c)) = y;
 }
 
 }  // namespace hattn
@@ -273,21 +330,33 @@ __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
 hipError_t hattn_quant_few_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
   using namespace hattn;
   const dim3 grid((unsigned)((long)p.B * p.G * p.rblocks * p.splits));
-#define GO(E, DP) hipLaunchKernelGGL((quant_few_kernel<E, DP>), grid, dim3(256), 0, stream, p)
-  if (dtype == 1) {
-    if (p.D <= 64) GO(_Float16, 64);
-    else GO(_Float16, 128);
-  } else {
-    if (p.D <= 64) GO(__bf16, 64);
-    else GO(__bf16, 128);
+  const long queries = (long)p.T * (p.H / p.G);
+#define RUN(E, DP, NB, C) \
+  hipLaunchKernelGGL((quant_few_kernel<E, DP, NB, C>), grid, dim3(256), 0, stream, p)
+#define GO(E, DP)                             \
+  if (queries > 16) RUN(E, DP, 2, false);     \
+  else if (p.coming) RUN(E, DP, 1, true);     \
+  else RUN(E, DP, 1, false);
+#define PICK(E)   \
+  if (p.D <= 64) { \
+    GO(E, 64)     \
+  } else {        \
+    GO(E, 128)    \
   }
+  if (dtype == 1) {
+    PICK(_Float16)
+  } else {
+    PICK(__bf16)
+  }
+#undef PICK
 #undef GO
+#undef RUN
   return hipGetLastError();
 }
 
 hipError_t hattn_quant_join_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
   using namespace hattn;
-  const dim3 grid((unsigned)((long)p.B * p.T * p.H));
+  const dim3 grid((unsigned)((long)p.B * p.T * p.H), (p.D + 63) / 64);
   if (dtype == 1)
     hipLaunchKernelGGL((quant_join_kernel<_Float16>), grid, dim3(256), 0, stream, p);
   else

@@ -9,7 +9,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from hattention import _lib
 
@@ -104,26 +103,31 @@ def _launch(q, k, freqs, positions, interleaved, scale, inverse):
 
 
 class RotaryFunction(torch.autograd.Function):
-    """(q, k) of :func:`rotary_embedding`; the backward turns the gradients back."""
+    """(q, k) of :func:`rotary_embedding`; the backward turns the gradients back, and can itself be
+    differentiated."""
 
     @staticmethod
-    def forward(ctx, q, k, freqs, positions, interleaved, scale):
+    def forward(ctx, q, k, freqs, positions, interleaved, scale, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(freqs, positions)
-        ctx.cfg = interleaved, scale
-        return _launch(q, k, freqs, positions, interleaved, scale, False)
+        ctx.cfg = interleaved, scale, inverse
+        return _launch(q, k, freqs, positions, interleaved, scale, inverse)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dq, dk):
         freqs, positions = ctx.saved_tensors
+        interleaved, scale, inverse = ctx.cfg
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
-        if dq is not None:
-            dq, dk = _launch(dq, dk, freqs, positions, *ctx.cfg, True)
-        elif dk is not None:
-            dk, _ = _launch(dk, None, freqs, positions, *ctx.cfg, True)
-        return dq, dk, None, None, None, None
+        if dq is not None or dk is not None:
+            # grad mode is on where the gradient's own gradient is wanted
+            turn = RotaryFunction.apply if torch.is_grad_enabled() else _launch
+            args = freqs, positions, interleaved, scale, not inverse
+            if dq is not None:
+                dq, dk = turn(dq, dk, *args)
+            else:
+                dk, _ = turn(dk, None, *args)
+        return dq, dk, None, None, None, None, None
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Tensor,
@@ -172,7 +176,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Te
     _lib.require_device(q, k, freqs, positions)
     if not freqs.is_contiguous():
         freqs = freqs.contiguous()
-    args = q, k, freqs, positions, layout == "interleaved", float(scale)
+    args = q, k, freqs, positions, layout == "interleaved", float(scale), False
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return RotaryFunction.apply(*args)
-    return _launch(*args, False)
+    return _launch(*args)

@@ -173,6 +173,21 @@ def test_which_gradients():
     assert none is None and torch.equal(torch.autograd.grad(y.sum(), x)[0], dq)
 
 
+def test_gradient_of_the_gradient():
+    """The gradient turns back, its own gradient forth."""
+    q, k = make(1, 2, 5, 2, 32, dtype=FS).requires_grad_(), make(2, 2, 5, 1, 32, dtype=FS).requires_grad_()
+    g = [t.detach().clone().requires_grad_() for t in (make(3, 2, 5, 2, 32, dtype=FS),
+                                                        make(4, 2, 5, 1, 32, dtype=FS))]
+    freqs, _ = rotary_frequencies(32, device=DEV)
+    y = rotary_embedding(q, k, freqs, None, "half", 1.5)
+    d = torch.autograd.grad(y, [q, k], g, create_graph=True)
+    h = [make(5, 2, 5, 2, 32, dtype=FS), make(6, 2, 5, 1, 32, dtype=FS)]
+    dd = torch.autograd.grad(d, g, h)
+    at = torch.arange(5, device=DEV).expand(2, 5)
+    for i in range(2):
+        close(dd[i], *oracle(h[i], freqs, at, "half", 1.5))
+
+
 def test_gradient_against_differences():
     """The map is linear, so its difference along any direction is the gradient along it."""
     q = make(1, 1, 6, 2, 32, dtype=FS).requires_grad_()

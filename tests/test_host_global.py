@@ -229,7 +229,7 @@ def test_alignment_strides_and_workspace_codes():
                                     *dims, 1.0, 0, ws, n, None)
     good = s(1024, 256, 64)
     need = _lib.load().hattn_quant_cache_attention_workspace(*dims)
-    assert need == 4 * 4 * 1 * 66 * 4
+    assert need == 4 * 4 * 1 * 66 * 4 + 4
     assert att(72, good, p, need) == VAL
     assert att(p, s(1024, 252, 64), p, need) == VAL
     assert att(p, s(1024, -256, 64), p, need) == VAL
@@ -249,7 +249,7 @@ def test_alignment_strides_and_workspace_codes():
 def test_workspace_query():
     f = _lib.load().hattn_quant_cache_attention_workspace
     # few queries: parts of at least 256 tokens, at most 256 of them, as many as fill the card
-    assert f(1, 1, 4, 4, 64, 256) == 4 * 1 * 66 * 4
-    assert f(1, 1, 4, 4, 64, 64 * 1024) == 4 * 256 * 66 * 4
+    assert f(1, 1, 4, 4, 64, 256) == 4 * 1 * 66 * 4 + 4
+    assert f(1, 1, 4, 4, 64, 64 * 1024) == 4 * 256 * 66 * 4 + 4
     assert f(0, 1, 4, 4, 64, 256) == 0
     assert f(1, 1, 4, 4, 60, 256) == 0
