@@ -97,6 +97,8 @@ Cut cut(int B, int T, int H, int G, int capacity) {
   return c;
 }
 
+bool joins(const Cut& c) { return c.few || c.splits > 1; }
+
 int attention_checks(int B, int T, int H, int G, int D, int capacity, float scale, int dtype) {
   if (T <= 0 || H <= 0) return fail(HATTN_ERR_VALUE, "non-positive dimension");
   if (int st = cache_checks(B, G, D, capacity)) return st;
@@ -106,12 +108,11 @@ int attention_checks(int B, int T, int H, int G, int D, int capacity, float scal
   if ((double)T * (H / G) > (double)(INT_MAX / 2))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "T=%d H=%d: 2^30 queries of a key head or more", T, H);
   const Cut c = cut(B, T, H, G, capacity);
-  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) || !fits((double)B * T * H, 512))
+  if (!fits((double)B * G * c.rblocks * c.splits + 8, 256) ||
+      (joins(c) && !fits((double)B * T * H, 512)))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d H=%d: 2^24 workgroups or more", B, T, H);
   return HATTN_OK;
 }
-
-bool joins(const Cut& c) { return c.few || c.splits > 1; }
 
 // Workspace in floats: the parts, their maxima and sums, and the rows' tokens during a step.
 size_t part_floats(int B, int T, int H, const Cut& c, int D) { return (size_t)B * T * H * c.splits * D; }
@@ -194,9 +195,10 @@ int hattn_rotary(const void* q, const void* k, const long long* strides, void* q
   while (p.cols < lanes) p.cols *= 2;
   // One round of kAhead heads a lane, so that many workgroups, in their several phases, share a CU
   // (4 x 8192 tokens of 32 heads of 64 in bf16: 55 us; with twice the tokens 60, half of them 56),
-  // but at least 1024 workgroups where the tokens allow it, and sines of at most 8 KB.
+  // but at least 1024 workgroups where the tokens allow it, and sines of at most 8 KB.  Single
+  // elements take four rounds (2 x 16384 tokens of 9 heads of 82: 52 us, with one 68).
   const long heads = (long)H + G;
-  p.tokens = (int)std::max(1L, std::min({512 / (heads * p.cols), (long)(1024 / pairs), p.N / 1024}));
+  p.tokens = (int)std::max(1L, std::min({(wide ? 512 : 2048) / (heads * p.cols), (long)(1024 / pairs), p.N / 1024}));
   if (!fits(std::ceil((double)p.N / p.tokens), 256))
     return fail(HATTN_ERR_NOT_IMPLEMENTED, "B=%d T=%d: 2^24 workgroups or more", B, T);
   return check_hip(hattn_rotary_launch(p, dtype, interleaved != 0, wide, (hipStream_t)stream),

@@ -6,8 +6,9 @@ Drop-in for the reference package's chunkwise entry points
 ``hattention.gated_delta_rule_apis.chunk_h_gated_delta_rule``), backed by the
 hand-written gfx950 kernels of ``libhattn_hip.so``.  Next to them a hybrid stack's
 other operators: ``hattention.sliding_apis`` (sliding-window attention with sinks),
-``hattention.recurrence_apis`` (a gated linear recurrence) and
-``hattention.norm_apis`` (layer norm with the residual stream's sum).
+``hattention.recurrence_apis`` (a gated linear recurrence), ``hattention.norm_apis``
+(layer norm with the residual stream's sum), ``hattention.rotary_apis`` (rotary
+positions) and ``hattention.quant_cache_apis`` (global attention over a cache in 8 bits).
 """
 from hattention.base import HType, HStruct, get_num_levels, ceil_log, floor_log
 

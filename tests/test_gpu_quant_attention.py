@@ -134,6 +134,26 @@ def test_scales_far_apart(dtype, T):
     close(quant_cache_attention(cache, q, 0.01), *oracle(cache, q, [500], [T], 0.01))
 
 
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("T", [1, 160])
+def test_many_tokens_of_little_weight(dtype, T):
+    """One token of weight 1 and 60000 of 2^-24 each, whose values are 2^7 times as large: their part
+    of the sum is lost where such weights are rounded to subnormal numbers."""
+    n, D = 60000, 64
+    slots = -(-n // BLOCK) * BLOCK
+    k = torch.zeros(1, 1, slots, D, device=DEV)
+    v = torch.full((1, 1, slots, D), 448.0, device=DEV)
+    k[0, 0, 5, 0] = 1.0
+    v[0, 0, 5] = 3.5
+    one = torch.ones(1, 1, slots // BLOCK, device=DEV)
+    cache = QuantCache(k.to(E4M3), v.to(E4M3), one, one.clone(),
+                       torch.tensor([n], dtype=torch.int32, device=DEV))
+    q = torch.zeros(1, T, 1, D, dtype=dtype, device=DEV)
+    q[..., 0] = 24.6
+    o = quant_cache_attention(cache, q, math.log(2))
+    close(o, *oracle(cache, q, [n], [T], math.log(2)))
+
+
 @pytest.mark.parametrize("T", [1, 64])
 def test_large_scores(T):
     """Scores of thousands, of both signs: one token takes all, which need not be the last seen."""
@@ -151,7 +171,8 @@ def test_large_scores(T):
 @pytest.mark.parametrize("dtype", [BF, FH])
 @pytest.mark.parametrize("B,H,G,D,start", [
     (1, 1, 1, 16, [0]), (3, 8, 2, 64, [0, 63, 640]), (2, 16, 16, 128, [127, 5]), (2, 34, 2, 80, [300, 64]),
-    (5, 6, 1, 112, [1, 2, 3, 4, 1000])])
+    (5, 6, 1, 112, [1, 2, 3, 4, 1000]), (2, 17, 1, 64, [64, 0]), (1, 66, 2, 128, [700]),
+    (2, 130, 1, 64, [90, 1])])
 def test_step(dtype, B, H, G, D, start):
     """Each step as append and attention, bit for bit, and near the formula."""
     a = filled(9, B, G, 1088, D, start)

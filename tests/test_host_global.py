@@ -218,7 +218,9 @@ def test_more_codes():
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert att(1, 4, 4, 2, 64, 128, scale) == VAL
     assert att(1, 2 ** 30, 64, 2, 64, 128, 1.0) == NOT
-    assert att(2 ** 12, 2 ** 12, 16, 1, 64, 128, 1.0) == NOT
+    assert att(2 ** 13, 2 ** 13, 32, 1, 64, 128, 1.0) == NOT
+    # a long prompt's queries are more than a join takes, which it does not need
+    assert att(1, 2 ** 18, 64, 8, 64, 2 ** 18, 1.0) == VAL
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="passes placeholder device pointers")
