@@ -74,7 +74,9 @@ QuantArgs cache_args(const void* kc, const void* vc, const float* ks, const floa
 // Blocks that T tokens from any place on can touch.
 int touched(int T) { return (T + kQuantBlock - 2) / kQuantBlock + 1; }
 
-// How a call's queries are cut: blocks of 16 or 32 where a row and key head has at most kFewQueries,
+// How a call's queries are cut: blocks of 16 or 32 where a row and key head has at most kFewQueries
+// (4 rows of up to 32000 tokens, 8 key heads of 128: 64 queries take 64 us so and 87 as part of
+// a block of 128, 128 queries 115 and 101),
 // else of 128; and parts of a row's tokens, enough that the card has work.  With few rows a workgroup's
 // start counts, and 1024 of them (512 with two blocks of queries each) are best: 4 rows of 8000
 // to 32000 tokens, 8 key heads of 128: 43 us with 1024, 46 with 2048, 52 with 4096.  With many rows,
@@ -83,7 +85,7 @@ struct Cut {
   bool few;
   int rblocks, splits;
 };
-const int kFewQueries = 128;
+const int kFewQueries = 64;
 Cut cut(int B, int T, int H, int G, int capacity) {
   Cut c;
   const long queries = (long)T * (H / G);

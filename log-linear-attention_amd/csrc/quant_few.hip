@@ -307,8 +307,8 @@ __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k, 64);
   __syncthreads();
-  // up to 64 elements a workgroup
-  const int c0 = blockIdx.y * 16, pieces = min(p.D / 4 - c0, 16), groups = 256 / pieces;
+  const int per = 32 / gridDim.y, c0 = blockIdx.y * per;
+  const int pieces = min(p.D / 4 - c0, per), groups = 256 / pieces;
   const int group = threadIdx.x / (unsigned)pieces, c = threadIdx.x - group * pieces;
   floatx4 x = zero4();
   if (group < groups) {
@@ -361,7 +361,9 @@ hipError_t hattn_quant_few_launch(const QuantArgs& p, int dtype, hipStream_t str
 
 hipError_t hattn_quant_join_launch(const QuantArgs& p, int dtype, hipStream_t stream) {
   using namespace hattn;
-  const dim3 grid((unsigned)((long)p.B * p.T * p.H), (p.D + 63) / 64);
+  // where there are many parts, 64 elements a workgroup (256 parts of 32 queries: 6.6 us, with all
+  // 128 elements 8.2; 4 parts of 2048 queries: 9.8, with all 6.2)
+  const dim3 grid((unsigned)((long)p.B * p.T * p.H), p.D > 64 && p.splits > 32 ? 2 : 1);
   if (dtype == 1)
     hipLaunchKernelGGL((quant_join_kernel<_Float16>), grid, dim3(256), 0, stream, p);
   else

@@ -80,7 +80,7 @@ SIZES = [  # B, T, H, G, D, counts, lengths
     (2, 1, 8, 2, 64, [700, 64], None),
     (3, 1, 16, 1, 128, [65, 1000, 4], [1, 1, 0]),
     (2, 1, 40, 2, 80, [513, 255], None),           # 20 queries of a key head
-    (2, 1, 33, 1, 128, [300, 129], None),          # 33, three blocks of 16, or one of 128
+    (2, 1, 33, 1, 128, [300, 129], None),          # 33, two blocks of 32
     (2, 5, 8, 2, 64, [900, 6], [5, 3]),
     (2, 4, 4, 1, 96, [4, 2], None),                # fewer tokens than queries: some see nothing
     (1, 8, 4, 1, 128, [64], None),                 # 32
@@ -89,6 +89,8 @@ SIZES = [  # B, T, H, G, D, counts, lengths
     (1, 300, 6, 2, 64, [300], None),               # a prompt
     (3, 129, 2, 1, 128, [129, 700, 40], [129, 1, 0]),
     (2, 70, 3, 3, 112, [1000, 70], [70, 70]),
+    (2, 16, 4, 1, 128, [200, 64], None),           # 64
+    (2, 13, 5, 1, 64, [200, 64], [13, 2]),         # 65
     (1, 64, 16, 1, 128, [3000], None),
     (4, 33, 8, 8, 32, [33, 64, 65, 500], [33, 32, 1, 17]),
 ]
