@@ -217,7 +217,7 @@ def test_full_and_empty_rows(H):
 
 
 def test_what_is_not_finite():
-    """NaN in k or v of a token reaches the queries that see it, and no block before theirs."""
+    """NaN in k or v of the last token reaches the last query."""
     for T in (2, 80):
         cache = filled(14, 1, 1, 256, 64, [256])
         q = make(15, 1, T, 2, 64)
@@ -239,6 +239,28 @@ def test_what_is_not_finite():
         o = quant_cache_attention(cache, q)
         assert o[0, 0, 1].isnan().all() and torch.equal(o[0, 1:], clean[0, 1:])
         assert torch.equal(o[0, 0, 0], clean[0, 0, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF, FH])
+@pytest.mark.parametrize("T,R", [(40, 2), (80, 2), (70, 5), (300, 1)])
+def test_how_far_a_nan_reaches(dtype, T, R):
+    """A NaN in v: to every query that sees it, and no further than the aligned 32 of which one
+    sees a token of its block."""
+    n, at = 400, 397
+    cache = filled(25, 1, 1, 448, 64, [n])
+    q = make(26, 1, T, R, 64, dtype=dtype)
+    clean = quant_cache_attention(cache, q)[0].flatten(0, 1)
+    cache.v.view(torch.uint8)[0, 0, at, 9] = 0x7f
+    o = quant_cache_attention(cache, q)[0].flatten(0, 1)
+    last = n - T + torch.arange(T * R, device=DEV) // R
+    assert o[last >= at, 9].isnan().all()
+    group = torch.arange(T * R, device=DEV) // 32
+    near = torch.zeros(int(group[-1]) + 1, dtype=torch.int64, device=DEV)
+    near = near.scatter_reduce(0, group, last, "amax")[group] >= at // BLOCK * BLOCK
+    assert near.any() and not near.all()
+    assert torch.equal(o[~near], clean[~near])
+    o[:, 9] = clean[:, 9] = 0
+    assert torch.equal(o, clean)
 
 
 @pytest.mark.parametrize("T", [3, 50])
