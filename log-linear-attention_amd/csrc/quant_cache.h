@@ -16,7 +16,7 @@ struct QuantArgs {
   int* counts;                    // [B]: tokens that each row has had
   void *o, *ko, *vo;              // o [B, T, H, D]; read: ko, vo [B, n, G, D]
   float *part, *stat;             // [B, T, H, splits, D], [B, T, H, splits, 2]
-  int* held;                      // [B], where `coming`: tokens with the new one, or -1 where it has no slot
+  int* held;                      // [B], where `coming`: tokens with the new one, -1 without a slot
   int B, T, H, G, D, cap;
   int start, n;                   // read: slots [start, start + n)
   int blocks;                     // append, read: blocks of a row, at most

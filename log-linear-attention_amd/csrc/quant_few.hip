@@ -6,8 +6,8 @@
 // on the codes themselves, which are exact in 16 bits: the scale ks of a block of keys multiplies
 // its scores, and vs the block's part of the sum.  P is rounded to the inputs' type.
 //
-// The cache is read once, which bounds it: 64 rows of up to 9000 tokens, 32 heads of 128 in 8 groups, 118
-// us (5.1 TB/s); one row of 262000, 4 key heads, 50 us (5.4 TB/s).  A row's slots are cut over
+// The cache is read once, which bounds it: 64 rows of up to 9000 tokens, 32 heads of 128 in 8 groups, 114
+// us (5.3 TB/s); one row of 262000, 4 key heads, 50 us (5.4 TB/s).  A row's slots are cut over
 // workgroups (by its own count, read on the device), whose partial results a second kernel joins
 // (6 to 8 us); a wave walks blocks of 64 slots, which have one scale, the next block's bytes in
 // flight.  Both K and V come straight into registers, K in 16 bytes of a slot's row a lane (two
@@ -15,8 +15,8 @@
 // which become operands over the slots by byte permutations.  No wave waits for another before
 // the end.
 //
-// A step's token is taken in by the one wave that walks its block, before its walk: a launch of its own
-// took 3 to 5 us.
+// A step's token is taken in by the one wave that walks its block, before its walk: a launch of
+// its own took 3 to 5 us.
 #include "quant_device.h"
 
 namespace hattn {
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
   }
-  const int first = rb * 16 * NB, least = row.end((unsigned)first / (unsigned)R);  // the first query sees least
+  const int first = rb * 16 * NB, least = row.end((unsigned)first / (unsigned)R);  // its first query's
 
   int end[NB];
   bf16x8 qf[NB][W][2];
