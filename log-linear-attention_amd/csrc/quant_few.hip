@@ -50,8 +50,13 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
   // for the join, which advances the counts
   if (COMING && split == 0 && g == 0 && threadIdx.x == 0) p.held[b] = row.full ? -1 : row.n;
   const int each = part_tokens(row.n, p.splits);
-  const int from = (int)min((long)split * each, (long)row.n), to = min(from + each, row.n);
-  if (from >= to) return;  // nor does the join read it
+  const int from = (int)min((long)split * each, (long)row.n);
+  const int first = rb * 16 * NB, last = min(first + 16 * NB, row.fresh * R) - 1;
+  // nor does the join read parts without tokens, and queries of padding
+  if (from >= row.n || first > last) return;
+  const int least = row.end((unsigned)first / (unsigned)R);  // its first query's
+  // Up to what the last one sees; a part behind that holds nothing, which the join reads.
+  const int to = min(from + each, row.end((unsigned)last / (unsigned)R));
   if constexpr (COMING) {
     // by the wave that walks the new token's block, which no other reads
     if (to == row.n && ((to - 1 - from) / kQuantBlock & 3) == wave) {
@@ -59,7 +64,6 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
   }
-  const int first = rb * 16 * NB, least = row.end((unsigned)first / (unsigned)R);  // its first query's
 
   int end[NB];
   bf16x8 qf[NB][W][2];
