@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
     };
     const auto part = [&](auto MASK, int s0, const __bf16* K, const __bf16* V)
                           __attribute__((always_inline)) {
-      const float unit = kscale * p.scale2;
+      float unit = kscale * p.scale2;
       floatx16 s[2];
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -125,13 +125,15 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
 #pragma unroll
         for (int c = 0; c < DP / 16; ++c) s[h] = mfma32<E>(kf[c], qf[c], s[h]);
       }
-      if constexpr (MASK.value) {
+      if constexpr (MASK.value) {  // behind the product with unit, which may be 0
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int up = end - s0 - 32 * h - 4 * hf;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[h][i] = 8 * (i >> 2) + (i & 3) < up ? s[h][i] : -INFINITY;
+          for (int i = 0; i < 16; ++i)
+            s[h][i] = 8 * (i >> 2) + (i & 3) < up ? s[h][i] * unit : -INFINITY;
         }
+        unit = 1.f;
       }
       __builtin_amdgcn_s_setprio(0);
       float top = fmaxf(s[0][0], s[0][1]);
