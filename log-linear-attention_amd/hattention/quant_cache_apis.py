@@ -55,10 +55,25 @@ class QuantCache:
     tokens, or to 0 to take a row into use again).  Tokens past the capacity are counted but not stored, and
     attention gives NaN for such a row."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "counts")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "counts", "_layout")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
                  v_scale: torch.Tensor, counts: torch.Tensor) -> None:
+        self.k, self.v, self.k_scale, self.v_scale, self.counts = k, v, k_scale, v_scale, counts
+        self._layout = None
+        self._check()
+        if (k.data_ptr() | v.data_ptr()) % 16:
+            raise ValueError("the cache must be aligned to 16 bytes")
+
+    def _check(self) -> None:
+        """That the tensors are what the kernels take: in each call, since the attributes can be set.
+        A layout that has passed is compared as a whole (2 us)."""
+        k, v, k_scale, v_scale, counts = self._tensors()
+        layout = (k.shape, v.shape, k_scale.shape, v_scale.shape, counts.shape, k.dtype, v.dtype,
+                  k_scale.dtype, v_scale.dtype, counts.dtype, k.is_contiguous(), v.is_contiguous(),
+                  k_scale.is_contiguous(), v_scale.is_contiguous(), counts.is_contiguous())
+        if layout == self._layout:
+            return
         if k.dim() != 4 or k.shape != v.shape or 0 in k.shape or k.shape[2] % BLOCK != 0 or \
                 k_scale.shape != (*k.shape[:2], k.shape[2] // BLOCK) or \
                 v_scale.shape != k_scale.shape or counts.shape != k.shape[:1]:
@@ -67,15 +82,13 @@ class QuantCache:
         if k.dtype != E4M3 or v.dtype != E4M3 or k_scale.dtype != torch.float32 or \
                 v_scale.dtype != torch.float32 or counts.dtype != torch.int32:
             raise ValueError("k and v must be float8_e4m3fn, the scales float32, counts int32")
-        if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale, counts)):
+        if not all(layout[10:]):
             raise ValueError("the cache must be contiguous: it is advanced in place")
-        if (k.data_ptr() | v.data_ptr()) % 16:
-            raise ValueError("the cache must be aligned to 16 bytes")
         if k.shape[3] % 16 != 0 or k.shape[3] > 128:
             raise NotImplementedError(f"D={k.shape[3]} is not a multiple of 16 up to 128")
         if k.shape[2] > MAX_CAPACITY:
             raise NotImplementedError(f"capacity={k.shape[2]} above {MAX_CAPACITY}")
-        self.k, self.v, self.k_scale, self.v_scale, self.counts = k, v, k_scale, v_scale, counts
+        self._layout = layout
 
     @classmethod
     def empty(cls, B: int, G: int, D: int, capacity: int, device="cuda") -> "QuantCache":
@@ -137,6 +150,7 @@ def quant_cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor,
     one; with ``lengths`` [B] (int32 or int64, on the device) the first lengths[b] of row b.  Keys enter
     with their positions applied.  Returns the cache, advanced in place; a captured call can be
     replayed (the counts are on the device)."""
+    cache._check()
     if k.dim() != 4 or 0 in k.shape:
         raise ValueError("k and v must be [B, T, G, D], not empty")
     B, T = k.shape[:2]
@@ -158,6 +172,7 @@ def quant_cache_read(cache: QuantCache, dtype: torch.dtype = torch.bfloat16, sta
     """Tokens start .. stop - 1 (to the capacity without ``stop``) of every row as k, v
     [B, stop - start, G, D] in bf16, fp16 or fp32, as :func:`quant_cache_append` took them; zero where a row
     has none."""
+    cache._check()
     B, G, slots, D = cache.k.shape
     stop = slots if stop is None else stop
     if not 0 <= start < stop <= slots:
@@ -185,6 +200,7 @@ def quant_cache_attention(cache: QuantCache, q: torch.Tensor, scale: Optional[fl
     Scores, softmax and sums are fp32; the probabilities are rounded to q's dtype between the products.
     Sums have a fixed order.  Without gradients.
     """
+    cache._check()
     if q.dim() != 4:
         raise ValueError("q must be [B, T, H, D]")
     scale = _check_queries(cache, q, scale)
@@ -208,6 +224,7 @@ def quant_cache_step(cache: QuantCache, q: torch.Tensor, k: torch.Tensor, v: tor
     and all before it: :func:`quant_cache_append` and :func:`quant_cache_attention` of T = 1 in one
     call, with the same results.  Returns (o [B, H, D], cache), the cache advanced in place; a captured step
     can be replayed."""
+    cache._check()
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError("q, k and v must be [B, heads, D]")
     scale = _check_queries(cache, q, scale)
