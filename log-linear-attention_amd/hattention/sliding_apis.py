@@ -147,10 +147,24 @@ class SlidingState:
     sinks + i the last token p >= sinks with p - sinks = i modulo window.  The step advances
     all three in place, on the device."""
 
-    __slots__ = ("k", "v", "counts", "window", "sinks")
+    __slots__ = ("k", "v", "counts", "window", "sinks", "_layout")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor, window: int,
                  sinks: int) -> None:
+        self.k, self.v, self.counts, self.window, self.sinks = k, v, counts, window, sinks
+        self._layout = None
+        self._check()
+        if (k.data_ptr() | v.data_ptr()) % 16:
+            raise ValueError("the cache must be aligned to 16 bytes")
+
+    def _check(self) -> None:
+        """That the tensors are what the kernel takes: in each step, since the attributes can be set.
+        A layout that has passed is compared as a whole."""
+        k, v, counts, window, sinks = self.k, self.v, self.counts, self.window, self.sinks
+        layout = (k.shape, v.shape, counts.shape, k.dtype, v.dtype, counts.dtype, k.is_contiguous(),
+                  v.is_contiguous(), counts.is_contiguous(), window, sinks)
+        if layout == self._layout:
+            return
         if k.dim() != 4 or k.shape != v.shape or k.shape[2] != sinks + window or \
                 counts.shape != (k.shape[0],):
             raise ValueError(f"cache of shapes {tuple(k.shape)}, {tuple(v.shape)}, "
@@ -159,9 +173,7 @@ class SlidingState:
             raise ValueError("k and v must have one dtype and counts be int32")
         if not (k.is_contiguous() and v.is_contiguous() and counts.is_contiguous()):
             raise ValueError("the cache must be contiguous: it is advanced in place")
-        if (k.data_ptr() | v.data_ptr()) % 16:
-            raise ValueError("the cache must be aligned to 16 bytes")
-        self.k, self.v, self.counts, self.window, self.sinks = k, v, counts, window, sinks
+        self._layout = layout
 
     @classmethod
     def empty(cls, B: int, G: int, D: int, window: int, sinks: int = 0,
@@ -200,6 +212,7 @@ def sliding_window_step(state: SlidingState, q: torch.Tensor, k: torch.Tensor, v
     advanced in place; a captured step can be replayed (the counts are on the device)."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("q, k and v must be [B, heads, D]")
+    state._check()
     window, sinks, kc = state.window, state.sinks, state.k
     scale = _check_shapes(q, k, v, window, sinks, scale)
     B, H, D = q.shape
