@@ -836,6 +836,8 @@ int hattn_quant_cache_read(const void* k_codes, const void* v_codes, const float
  * values; zero for t >= lengths[b] and where a query sees nothing, NaN in rows whose count has
  * passed the capacity.  A NaN in v of a token may reach a query that does not see it where one of the
  * query's aligned 32 (in the order t * (H / G) + head of the group) sees a token of the same 64.
+ * Sums over the weights stay finite for all values of v that the cache holds; in BF16 values below 2^-52 may
+ * count as 0 in rows that have values above 2^88.
  * step: one token a row, k, v [B, G, D], q, o [B, H, D] (strides as of T = 1: batch, token, head
  * of q, k, v): append, then attention.  Both: workspace
  * hattn_quant_cache_attention_workspace(B, T, ..) bytes (T = 1 for the step), aligned to 16,

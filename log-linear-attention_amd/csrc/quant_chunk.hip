@@ -18,7 +18,10 @@
 // A block of 64 slots has one scale of K, which multiplies its scores, and one of V, which is folded into
 // P's exponent.  In bf16 its range holds that.  In fp16 the sums are in units of a scale near
 // the block's own (at least 2^-40: smaller values are 0 in the result), so that P is folded by
-// at most 2^-8, which its lift makes up for.
+// at most 2^-8, which its lift makes up for.  In bf16 a workgroup that comes across a scale above 2^80 has its
+// sums in units of 2^40, so that they stay finite, and a loop of its own (a test in each tile costs 1 to
+// 2%).  Scales below 2^-60 are out of P's range there: their blocks count for the sum of the weights alone,
+// their values, below 2^-52, as 0.
 //
 // Where blocks are few, a row's slots are cut over workgroups too, whose partial results
 // quant_few.hip's second kernel joins.
@@ -38,7 +41,8 @@ struct Halves {
   }
 };
 
-constexpr float kLeastUnit = 0x1p-40f;
+constexpr float kLeastUnit = 0x1p-40f;                                 // fp16
+constexpr float kLarge = 0x1p80f, kUnit = 0x1p40f, kLeast = 0x1p-60f;  // bf16
 
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(QuantArgs p) {
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
       kscale = knext;
       vscale = vnext;
     };
-    const auto part = [&](auto MASK, int s0, const __bf16* K, const __bf16* V)
+    const auto part = [&](auto MASK, auto LARGE, int s0, const __bf16* K, const __bf16* V)
                           __attribute__((always_inline)) {
       float unit = kscale * p.scale2;
       floatx16 s[2];
@@ -157,7 +161,18 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
         for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= by;
         vunit = next;
       }
-      const float ratio = UNITS ? vscale * __builtin_amdgcn_rcpf(vunit) : vscale;
+      float ratio = UNITS ? vscale * __builtin_amdgcn_rcpf(vunit) : vscale;
+      if constexpr (LARGE.value) {
+        ratio *= 1.f / kUnit;
+        if (vscale < kLeast) {  // the weights' sum, and P = 0
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            l += exp2_(fmaf(s[0][i], unit, -m)) + exp2_(fmaf(s[1][i], unit, -m));
+            s[0][i] = s[1][i] = -INFINITY;
+          }
+          ratio = unit = 1.f;
+        }
+      }
       const float base = m - Half<E>::kLift - __builtin_amdgcn_logf(ratio);
       float sum = 0.f;
 #pragma unroll
@@ -178,25 +193,39 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
           acc[dt] = mfma32<E>(tr32<DP>(V, 16 * c, 32 * dt), pf[c], acc[dt]);
       __builtin_amdgcn_s_setprio(0);
     };
-    const auto step = [&](auto MASK, int s0, const __bf16* K, const __bf16* V, __bf16* Kn, __bf16* Vn)
-                          __attribute__((always_inline)) {
+    const auto step = [&](auto MASK, auto LARGE, int s0, const __bf16* K, const __bf16* V, __bf16* Kn,
+                          __bf16* Vn) __attribute__((always_inline)) {
       __syncthreads();
       const bool more = s0 + BN < to;
       if (more) fetch(s0 + BN);
-      if (!MASK.value || s0 < most) part(MASK, s0, K, V);
+      if (!MASK.value || s0 < most) part(MASK, LARGE, s0, K, V);
       if (more) put(Kn, Vn);
     };
+    float largest = 0.f;  // of the scales of V
+    if constexpr (!UNITS) {
+      const int end_block = (to - 1) / kQuantBlock;
+      int i = from / kQuantBlock + lane;
+      largest = vs[min(i, end_block)];
+      while ((i += 64) <= end_block) largest = fmaxf(largest, vs[i]);
+    }
     fetch(from);
     put(K0, V0);
+    const bool large = !UNITS && __any(largest > kLarge);
     int s0 = from;
-    const auto pair = [&](auto MASK) __attribute__((always_inline)) {
-      step(MASK, s0, K0, V0, K1, V1);
-      if (!MASK.value || s0 + BN < to) step(MASK, s0 + BN, K1, V1, K0, V0);
+    const auto pair = [&](auto MASK, auto LARGE) __attribute__((always_inline)) {
+      step(MASK, LARGE, s0, K0, V0, K1, V1);
+      if (!MASK.value || s0 + BN < to) step(MASK, LARGE, s0 + BN, K1, V1, K0, V0);
     };
-    // blocks that all queries see whole, in pairs, then those that need masks
-    for (const int whole = min(row.end(q0 / R), to); s0 + 2 * BN <= whole; s0 += 2 * BN)
-      pair(Bool<false>());
-    for (; s0 < to; s0 += 2 * BN) pair(Bool<true>());
+    if (!large) {
+      // blocks that all queries see whole, in pairs, then those that need masks
+      for (const int whole = min(row.end(q0 / R), to); s0 + 2 * BN <= whole; s0 += 2 * BN)
+        pair(Bool<false>(), Bool<false>());
+      for (; s0 < to; s0 += 2 * BN) pair(Bool<true>(), Bool<false>());
+    } else if constexpr (!UNITS) {
+      vunit = kUnit;
+      for (bool odd = false; s0 < to; s0 += BN, odd = !odd)
+        step(Bool<true>(), Bool<true>(), s0, odd ? K1 : K0, odd ? V1 : V0, odd ? K0 : K1, odd ? V0 : V1);
+    }
     const Halves both(l);
     l = both.lo + both.hi;
   }
@@ -225,7 +254,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void quant_chunk_kernel(Quan
       const int d = 32 * dt + 8 * i + 4 * hf;
       floatx4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * i + j] * vunit;
+      for (int j = 0; j < 4; ++j) x[j] = acc[dt][4 * i + j] * (vunit * Half<E>::kPart);
       if (d < p.D) *(floatx4*)(p.part + to_part * p.D + d) = x;
     }
   if (hf == 0) {

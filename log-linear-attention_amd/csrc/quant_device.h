@@ -23,19 +23,21 @@ template <>
 struct Half<__bf16> {
   static constexpr unsigned kInf = 0x7f80;
   static constexpr int kMost = 119;
-  static constexpr float kSlack = 8.f, kLift = 0.f;
+  static constexpr float kSlack = 8.f, kLift = 0.f, kPart = 0x1p-40f;
 };
 template <>
 struct Half<_Float16> {
   static constexpr unsigned kInf = 0x7c00;
   static constexpr int kMost = 7;
-  static constexpr float kSlack = 4.f, kLift = 11.f;
+  static constexpr float kSlack = 4.f, kLift = 11.f, kPart = 1.f;
 };
 
 // The running maximum m of a query's scores (powers of two) is taken again only where a score passes
 // it by more than kSlack, so that most tiles do not rescale the sums; probabilities are
 // 2^(s - m + kLift), at most 2^15.  In fp16 the lift keeps those down to 2^-25 of the largest out of
 // the subnormal numbers: of many tokens of little weight each, the sum would be off.
+// Weights of up to 2^kSlack of 2^30 tokens come to 2^38 before they are divided by their sum: in bf16,
+// whose values go to 2^128, partial results are held times kPart.
 
 // The magnitude of a 16-bit number as an integer of the same order; 0 where it is not finite.
 template <typename E>

@@ -192,6 +192,7 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
       pf[nb][0] = cat8e<E>(s[nb][0], s[nb][1]);
       pf[nb][1] = cat8e<E>(s[nb][2], s[nb][3]);
     }
+    const float unit_v = vscale * Half<E>::kPart;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       floatx4 o[NB][4];
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void quant_few_kernel(QuantArgs p) {
         for (int n = 0; n < 4; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            acc[nb][4 * w + n][i] = fmaf(o[nb][n][i], vscale, acc[nb][4 * w + n][i]);
+            acc[nb][4 * w + n][i] = fmaf(o[nb][n][i], unit_v, acc[nb][4 * w + n][i]);
     }
     if (s0 + 4 * kQuantBlock < to) load_v(s0 + 4 * kQuantBlock);
   }
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256) void quant_join_kernel(QuantArgs p) {
   for (int s = 1; s < min(groups, live); ++s) x += sums[s * pieces + c];
   bf16x4 y;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) y[i] = to16<E>(x[i] / sum);
+  for (int i = 0; i < 4; ++i) y[i] = to16<E>(x[i] / (sum * Half<E>::kPart));
   *(bf16x4*)(o + 4 * (c0 + c)) = y;
 }
 
