@@ -9,6 +9,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_native", "libhattn_hip.so")
@@ -160,6 +161,18 @@ def require_device(*tensors) -> torch.device:
             raise RuntimeError("tensors on different devices")
         dev = t.device
     return dev
+
+
+def wants_grad(*tensors) -> bool:
+    """Whether a call on these tensors goes through its autograd function: a backward may follow, or
+    one of them has a tangent of forward mode."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # the level is -1 outside of that mode; looked at first, since unpacking takes 0.5 us a tensor
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def ptr(t) -> int:

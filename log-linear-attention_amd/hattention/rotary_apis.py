@@ -102,16 +102,34 @@ def _launch(q, k, freqs, positions, interleaved, scale, inverse):
     return qo, ko
 
 
+def _turn(q, k, *args):
+    """:func:`_launch`, differentiable where that is wanted."""
+    return (RotaryFunction.apply if _lib.wants_grad(q, k) else _launch)(q, k, *args)
+
+
 class RotaryFunction(torch.autograd.Function):
     """(q, k) of :func:`rotary_embedding`; the backward turns the gradients back, and can itself be
-    differentiated."""
+    differentiated; tangents are turned as their tensors are."""
 
     @staticmethod
     def forward(ctx, q, k, freqs, positions, interleaved, scale, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(freqs, positions)
+        ctx.save_for_forward(freqs, positions)
         ctx.cfg = interleaved, scale, inverse
+        ctx.q_shape, ctx.k_shape = q.shape, None if k is None else k.shape
         return _launch(q, k, freqs, positions, interleaved, scale, inverse)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # of outputs that are tensors the engine takes zeros, not None
+        if tq is None:
+            tk, _ = _turn(tk, None, *ctx.saved_tensors, *ctx.cfg)
+            return torch.zeros(ctx.q_shape, dtype=tk.dtype, device=tk.device), tk
+        tq, tk = _turn(tq, tk, *ctx.saved_tensors, *ctx.cfg)
+        if tk is None and ctx.k_shape is not None:
+            tk = torch.zeros(ctx.k_shape, dtype=tq.dtype, device=tq.device)
+        return tq, tk
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -120,13 +138,11 @@ class RotaryFunction(torch.autograd.Function):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is not None or dk is not None:
-            # grad mode is on where the gradient's own gradient is wanted
-            turn = RotaryFunction.apply if torch.is_grad_enabled() else _launch
             args = freqs, positions, interleaved, scale, not inverse
             if dq is not None:
-                dq, dk = turn(dq, dk, *args)
+                dq, dk = _turn(dq, dk, *args)
             else:
-                dk, _ = turn(dk, None, *args)
+                dk, _ = _turn(dk, None, *args)
         return dq, dk, None, None, None, None, None
 
 
@@ -141,7 +157,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Te
     2 n <= D.  ``layout`` "half" pairs elements i and i + n, "interleaved" 2 i and 2 i + 1.
     ``positions`` (int32 or int64, on the device): [B], of each row's first token, or [B, T], of every
     token; None: 0 to T - 1 (one token a row needs [B]).  Returns (q, k), contiguous; gradients
-    reach q and k.
+    reach q and k, and so do tangents of forward mode; ``freqs`` that require a gradient are refused.
 
     Angles are taken and reduced in 64 bits, sines and products in 32, at any position.
     """
@@ -162,6 +178,8 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Te
         raise ValueError(f"freqs {tuple(freqs.shape)} for heads of {D}")
     if freqs.dtype not in (torch.float32, torch.float64):
         raise NotImplementedError(f"freqs in {freqs.dtype}")
+    if _lib.wants_grad(freqs):
+        raise NotImplementedError("freqs have no gradient: pass them detached")
     if D > MAX_D:
         raise NotImplementedError(f"D={D} above {MAX_D}")
     if not math.isfinite(scale) or abs(scale) > 1e30:
@@ -176,7 +194,4 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], freqs: torch.Te
     _lib.require_device(q, k, freqs, positions)
     if not freqs.is_contiguous():
         freqs = freqs.contiguous()
-    args = q, k, freqs, positions, layout == "interleaved", float(scale), False
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return RotaryFunction.apply(*args)
-    return _launch(*args)
+    return _turn(q, k, freqs, positions, layout == "interleaved", float(scale), False)
