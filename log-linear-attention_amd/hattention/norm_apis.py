@@ -117,8 +117,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
             raise NotImplementedError(f"residual in {residual.dtype} with x in {x.dtype}")
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+    if _lib.wants_grad(x, residual, weight, bias):
         y, s = LayerNormFunction.apply(x, residual, weight, bias, eps)
     else:
         y, s, _ = _forward(x, residual, weight, bias, eps, False)

@@ -123,8 +123,7 @@ def gated_linear_recurrence(x: torch.Tensor, g: torch.Tensor,
     lengths = check_lengths(lengths, B, dev)
     x, g = _aligned(x), _aligned(g)
     h0 = initial_state.float().contiguous() if initial_state is not None else None
-    if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad
-                                    or (h0 is not None and h0.requires_grad)):
+    if _lib.wants_grad(x, g, h0):
         o, ht = GatedRecurrenceFunction.apply(x, g, h0, lengths, output_final_state)
     else:
         o, ht, _ = _forward(x, g, h0, lengths, output_final_state, False)

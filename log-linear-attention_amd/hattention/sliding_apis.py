@@ -136,7 +136,7 @@ def sliding_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     lengths = check_lengths(lengths, q.shape[0], dev)
     q, k, v = _rows(q), _rows(k), _rows(v)
     window = min(window, q.shape[1])  # a window of T keys holds every earlier one
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _lib.wants_grad(q, k, v):
         return SlidingWindowFunction.apply(q, k, v, lengths, window, sinks, scale)
     return _forward(q, k, v, lengths, window, sinks, scale, False)[0]
 
