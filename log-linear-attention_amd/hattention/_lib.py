@@ -163,6 +163,12 @@ def require_device(*tensors) -> torch.device:
     return dev
 
 
+def advanced(*tensors) -> None:
+    """Tells autograd that a kernel changes these tensors in place, as torch's own operators do: a
+    backward that has kept one of them refuses then."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def wants_grad(*tensors) -> bool:
     """Whether a call on these tensors goes through its autograd function: a backward may follow, or
     one of them has a tangent of forward mode."""

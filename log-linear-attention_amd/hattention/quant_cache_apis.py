@@ -164,6 +164,7 @@ def quant_cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor,
     _lib.launch(dev, _lib.load().hattn_quant_cache_append, k.data_ptr(), v.data_ptr(),
                 _lib.ptr(lengths), _Strides6(*sk, *sv), *cache._ptrs(), B, T, k.shape[2], k.shape[3],
                 cache.capacity, _lib.dtype_code(k))
+    _lib.advanced(*cache._tensors())
     return cache
 
 
@@ -239,4 +240,5 @@ def quant_cache_step(cache: QuantCache, q: torch.Tensor, k: torch.Tensor, v: tor
     _lib.launch(dev, _lib.load().hattn_quant_cache_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 _Strides9(*sq, *sk, *sv), *cache._ptrs(), o.data_ptr(), B, H, G, D, slots, scale,
                 _lib.dtype_code(q), ws_ptr, ws_bytes)
+    _lib.advanced(*cache._tensors())
     return o, cache

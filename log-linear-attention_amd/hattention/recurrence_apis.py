@@ -150,4 +150,5 @@ def gated_linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, g: torch.
     B, D = x.shape
     _lib.launch(dev, _lib.load().hattn_gated_recurrence_step, state.data_ptr(), x.data_ptr(),
                 g.data_ptr(), o.data_ptr(), B, D, _lib.dtype_code(x), _lib.dtype_code(g))
+    _lib.advanced(state)
     return o, state

@@ -227,4 +227,5 @@ def sliding_window_step(state: SlidingState, q: torch.Tensor, k: torch.Tensor, v
     _lib.launch(dev, _lib.load().hattn_sliding_step, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 kc.data_ptr(), state.v.data_ptr(), state.counts.data_ptr(), o.data_ptr(), B, H, G,
                 D, window, sinks, scale, _lib.dtype_code(q), ws_ptr, ws_bytes)
+    _lib.advanced(kc, state.v, state.counts)
     return o, state
