@@ -169,6 +169,11 @@ def advanced(*tensors) -> None:
     torch.autograd.graph.increment_version(tensors)
 
 
+def forward_mode() -> bool:
+    """Whether tensors may have tangents: the mode's level is -1 where there are none."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def wants_grad(*tensors) -> bool:
     """Whether a call on these tensors goes through its autograd function: a backward may follow, or
     one of them has a tangent of forward mode."""
@@ -176,8 +181,8 @@ def wants_grad(*tensors) -> bool:
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    # the level is -1 outside of that mode; looked at first, since unpacking takes 0.5 us a tensor
-    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
+    # the mode first: unpacking takes 0.5 us a tensor
+    return forward_mode() and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 

@@ -115,9 +115,10 @@ class RotaryFunction(torch.autograd.Function):
     def forward(ctx, q, k, freqs, positions, interleaved, scale, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(freqs, positions)
-        ctx.save_for_forward(freqs, positions)
         ctx.cfg = interleaved, scale, inverse
-        ctx.q_shape, ctx.k_shape = q.shape, None if k is None else k.shape
+        if _lib.forward_mode():
+            ctx.save_for_forward(freqs, positions)
+            ctx.q_shape, ctx.k_shape = q.shape, None if k is None else k.shape
         return _launch(q, k, freqs, positions, interleaved, scale, inverse)
 
     @staticmethod
@@ -138,11 +139,13 @@ class RotaryFunction(torch.autograd.Function):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         if dq is not None or dk is not None:
+            # grad mode is on where the gradient's own gradient is wanted
+            turn = RotaryFunction.apply if torch.is_grad_enabled() or _lib.forward_mode() else _launch
             args = freqs, positions, interleaved, scale, not inverse
             if dq is not None:
-                dq, dk = _turn(dq, dk, *args)
+                dq, dk = turn(dq, dk, *args)
             else:
-                dk, _ = _turn(dk, None, *args)
+                dk, _ = turn(dk, None, *args)
         return dq, dk, None, None, None, None, None
 
 
