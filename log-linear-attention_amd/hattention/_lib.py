@@ -163,10 +163,14 @@ def require_device(*tensors) -> torch.device:
     return dev
 
 
+_increment_version = getattr(torch._C, "_increment_version",
+                             torch.autograd.graph.increment_version)
+
+
 def advanced(*tensors) -> None:
     """Tells autograd that a kernel changes these tensors in place, as torch's own operators do: a
     backward that has kept one of them refuses then."""
-    torch.autograd.graph.increment_version(tensors)
+    _increment_version(tensors)
 
 
 def forward_mode() -> bool:

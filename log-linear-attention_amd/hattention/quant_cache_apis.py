@@ -25,7 +25,11 @@ _Strides3, _Strides6, _Strides9 = (ctypes.c_longlong * n for n in (3, 6, 9))
 def _lead(t):
     """t, or a copy, with contiguous rows that start on 16 bytes, and its batch, token and head
     strides (0 where there is one element: torch leaves such a stride at any value)."""
-    s, n = t.stride(), t.shape
+    n = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        row = n[-2] * n[-1]
+        return t, (row, 0, n[-1]) if len(n) == 3 else (n[1] * row, row, n[-1])
+    s = t.stride()
     if len(n) == 3:  # one token a row
         lead = s[0] if n[0] > 1 else 0, 0, s[1] if n[1] > 1 else 0
     else:
@@ -67,11 +71,12 @@ class QuantCache:
 
     def _check(self) -> None:
         """That the tensors are what the kernels take: in each call, since the attributes can be set.
-        A layout that has passed is compared as a whole (2 us)."""
+        A layout that has passed is compared as a whole (0.7 us)."""
         k, v, k_scale, v_scale, counts = self._tensors()
         layout = (k.shape, v.shape, k_scale.shape, v_scale.shape, counts.shape, k.dtype, v.dtype,
                   k_scale.dtype, v_scale.dtype, counts.dtype, k.is_contiguous(), v.is_contiguous(),
-                  k_scale.is_contiguous(), v_scale.is_contiguous(), counts.is_contiguous())
+                  k_scale.is_contiguous(), v_scale.is_contiguous(), counts.is_contiguous(),
+                  k.device, v.device, k_scale.device, v_scale.device, counts.device)
         if layout == self._layout:
             return
         if k.dim() != 4 or k.shape != v.shape or 0 in k.shape or k.shape[2] % BLOCK != 0 or \
@@ -82,12 +87,14 @@ class QuantCache:
         if k.dtype != E4M3 or v.dtype != E4M3 or k_scale.dtype != torch.float32 or \
                 v_scale.dtype != torch.float32 or counts.dtype != torch.int32:
             raise ValueError("k and v must be float8_e4m3fn, the scales float32, counts int32")
-        if not all(layout[10:]):
+        if not all(layout[10:15]):
             raise ValueError("the cache must be contiguous: it is advanced in place")
         if k.shape[3] % 16 != 0 or k.shape[3] > 128:
             raise NotImplementedError(f"D={k.shape[3]} is not a multiple of 16 up to 128")
         if k.shape[2] > MAX_CAPACITY:
             raise NotImplementedError(f"capacity={k.shape[2]} above {MAX_CAPACITY}")
+        if len(set(layout[15:])) > 1:
+            raise RuntimeError("the cache's tensors are on different devices")
         self._layout = layout
 
     @classmethod
@@ -116,9 +123,10 @@ class QuantCache:
 
 def _check_half(*tensors) -> None:
     dtype = tensors[0].dtype
-    if any(t.dtype != dtype for t in tensors):
-        raise ValueError("q, k and v must have one dtype")
-    if dtype not in (torch.bfloat16, torch.float16):
+    for t in tensors:
+        if t.dtype is not dtype:
+            raise ValueError("q, k and v must have one dtype")
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise NotImplementedError(f"{dtype}: bf16 or fp16 only")
 
 
@@ -158,7 +166,7 @@ def quant_cache_append(cache: QuantCache, k: torch.Tensor, v: torch.Tensor,
     _check_half(k, v)
     if T > cache.capacity:
         raise ValueError(f"T={T} tokens for a capacity of {cache.capacity}")
-    dev = _lib.require_device(k, v, *cache._tensors())
+    dev = _lib.require_device(cache.k, k, v)
     lengths = check_lengths(lengths, B, dev)
     (k, sk), (v, sv) = _lead(k), _lead(v)
     _lib.launch(dev, _lib.load().hattn_quant_cache_append, k.data_ptr(), v.data_ptr(),
@@ -180,7 +188,7 @@ def quant_cache_read(cache: QuantCache, dtype: torch.dtype = torch.bfloat16, sta
         raise ValueError(f"tokens {start} to {stop} of {slots}")
     if dtype not in _lib.DTYPE_CODES:
         raise NotImplementedError(f"unsupported dtype {dtype}")
-    dev = _lib.require_device(*cache._tensors())
+    dev = _lib.require_device(cache.k)
     k, v = (torch.empty(B, stop - start, G, D, dtype=dtype, device=dev) for _ in range(2))
     _lib.launch(dev, _lib.load().hattn_quant_cache_read, *cache._ptrs(), k.data_ptr(), v.data_ptr(),
                 B, G, D, slots, start, stop - start, _lib.DTYPE_CODES[dtype])
@@ -206,7 +214,7 @@ def quant_cache_attention(cache: QuantCache, q: torch.Tensor, scale: Optional[fl
         raise ValueError("q must be [B, T, H, D]")
     scale = _check_queries(cache, q, scale)
     _check_half(q)
-    dev = _lib.require_device(q, *cache._tensors())
+    dev = _lib.require_device(cache.k, q)
     B, T, H, D = q.shape
     lengths = check_lengths(lengths, B, dev)
     q, sq = _lead(q)
@@ -231,7 +239,7 @@ def quant_cache_step(cache: QuantCache, q: torch.Tensor, k: torch.Tensor, v: tor
     scale = _check_queries(cache, q, scale)
     _check_new(cache, k, v, ())
     _check_half(q, k, v)
-    dev = _lib.require_device(q, k, v, *cache._tensors())
+    dev = _lib.require_device(cache.k, q, k, v)
     B, H, D = q.shape
     (q, sq), (k, sk), (v, sv) = _lead(q), _lead(k), _lead(v)
     o = torch.empty(B, H, D, dtype=q.dtype, device=dev)
