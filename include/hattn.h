@@ -816,7 +816,10 @@ int hattn_rotary(const void* q, const void* k, const long long* strides, void* q
  * append: tokens k, v [B, T, G, D] (strides: batch, token, head of k, then v, in elements,
  * multiples of 8; aligned to 16 bytes) in BF16 or FP16 enter after those that are there, of row b
  * the first lengths[b] (clamped to [0, T]; NULL: T).  counts advance on the device, past the capacity
- * too: those tokens are not stored.  A count may be set back: what is there stays usable up to it.
+ * too: those tokens are not stored.  A count may be set back: what is there stays usable up to it.  Into
+ * the middle of a block, that block's scale stays the largest that any of its tokens has needed, the
+ * dropped ones among them, and the codes that they made smaller stay so: to go back exactly, a caller
+ * keeps the block's codes and scales.
  *
  * read: slots [start, start + n) as k, v [B, n, G, D] contiguous, in any dtype, zero where a
  * row has no token.
@@ -837,7 +840,7 @@ int hattn_quant_cache_read(const void* k_codes, const void* v_codes, const float
  * passed the capacity.  A NaN in v of a token may reach a query that does not see it where one of the
  * query's aligned 32 (in the order t * (H / G) + head of the group) sees a token of the same 64.
  * Sums over the weights stay finite for all values of v that the cache holds; in BF16 values below 2^-52 may
- * count as 0 in rows that have values above 2^88.
+ * count as 0 in rows that have values above 2^88.  q in FP16 expects values in that type's range.
  * step: one token a row, k, v [B, G, D], q, o [B, H, D] (strides as of T = 1: batch, token, head
  * of q, k, v): append, then attention.  Both: workspace
  * hattn_quant_cache_attention_workspace(B, T, ..) bytes (T = 1 for the step), aligned to 16,

@@ -75,8 +75,8 @@ QuantArgs cache_args(const void* kc, const void* vc, const float* ks, const floa
 int touched(int T) { return (T + kQuantBlock - 2) / kQuantBlock + 1; }
 
 // How a call's queries are cut: blocks of 16 or 32 where a row and key head has at most kFewQueries
-// (4 rows of up to 32000 tokens, 8 key heads of 128: 64 queries take 64 us so and 87 as part of
-// a block of 128, 128 queries 115 and 101),
+// (4 rows of up to 32000 tokens, 8 key heads of 128: 64 queries take 63 us so and 87 as part of
+// a block of 128, 128 queries 115 and 90),
 // else of 128; and parts of a row's tokens, enough that the card has work.  With few rows a workgroup's
 // start counts, and 1024 of them (512 with two blocks of queries each) are best: 4 rows of 8000
 // to 32000 tokens, 8 key heads of 128: 43 us with 1024, 46 with 2048, 52 with 4096.  With many rows,
@@ -196,7 +196,7 @@ int hattn_rotary(const void* q, const void* k, const long long* strides, void* q
   p.cols = 1;
   while (p.cols < lanes) p.cols *= 2;
   // One round of kAhead heads a lane, so that many workgroups, in their several phases, share a CU
-  // (4 x 8192 tokens of 32 heads of 64 in bf16: 55 us; with twice the tokens 60, half of them 56),
+  // (4 x 8192 tokens of 32 heads of 64 in bf16: 53 us; with twice the tokens 5 more, half of them 1),
   // but at least 1024 workgroups where the tokens allow it, and sines of at most 8 KB.  Single
   // elements take four rounds (2 x 16384 tokens of 9 heads of 82: 52 us, with one 68).
   const long heads = (long)H + G;

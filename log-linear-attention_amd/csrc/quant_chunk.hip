@@ -9,11 +9,13 @@
 // registers that its bytes come to, one tile ahead, and LDS, in the layout of sliding_device.h.
 // Tiles that all of the block's queries see whole have a loop without masks.
 //
-// The matrix products bound it, and the softmax's vector instructions beside them where D is 64: 2048
-// queries of 32 heads of 128 after 30000 tokens take 956 us (1.09 PFLOP/s, of the 1.2 that a large
-// product reaches), 4 prompts of up to 4005 tokens of 16 heads of 64 149 us (0.60 PFLOP/s).  Tiles
-// of 32, with a barrier each, took 1052 us; waves take priority during their products: without
-// that 1010 us.
+// 2048 queries of 32 heads of 128 after 30000 tokens take 931 to 954 us (1.12 to 1.09 PFLOP/s, of the 1.2
+// that a large product reaches): the matrix units are busy in 53% of the cycles and the vector units, with
+// the softmax, in 40%, at the clock that the card's power leaves.  In fp16 1012 us.  With heads of 64 608 us (0.86
+// PFLOP/s; 36% and 49%), and 4 prompts of up to 4005 tokens of 16 heads of 64 149 us (0.60 PFLOP/s):
+// there a CU has work for 60% of the time.  D = 80, 96 and 112 run the products of 128: 904 us and 917
+// for the first two.  Tiles of 32, with a barrier each, took a tenth more; waves take priority during their
+// products: without that 5% more.
 //
 // A block of 64 slots has one scale of K, which multiplies its scores, and one of V, which is folded into
 // P's exponent.  In bf16 its range holds that.  In fp16 the sums are in units of a scale near

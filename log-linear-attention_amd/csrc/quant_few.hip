@@ -6,8 +6,8 @@
 // on the codes themselves, which are exact in 16 bits: the scale ks of a block of keys multiplies
 // its scores, and vs the block's part of the sum.  P is rounded to the inputs' type.
 //
-// The cache is read once, which bounds it: 64 rows of up to 9000 tokens, 32 heads of 128 in 8 groups, 114
-// us (5.3 TB/s); one row of 262000, 4 key heads, 50 us (5.4 TB/s).  A row's slots are cut over
+// The cache is read once, which bounds it: 64 rows of up to 9000 tokens, 32 heads of 128 in 8 groups, 115
+// us (5.2 TB/s); one row of 262000, 4 key heads, 50 us (5.3 TB/s).  A row's slots are cut over
 // workgroups (by its own count, read on the device), whose partial results a second kernel joins
 // (6 to 8 us); a wave walks blocks of 64 slots, which have one scale, the next block's bytes in
 // flight.  Both K and V come straight into registers, K in 16 bytes of a slot's row a lane (two

@@ -8,11 +8,11 @@
 // to 32: at position 10^6 an angle in 32 bits would be off by 0.06.
 //
 // Each element is read and written once, which bounds it: 4 x 8192 tokens of 32 heads of 64 in bf16 take
-// 50 us (5.4 TB/s), 32768 tokens of 40 heads of 128 114 us (5.9 TB/s).  The sines of a workgroup's tokens
+// 53 us (5.0 TB/s), 32768 tokens of 40 heads of 128 114 us (5.9 TB/s).  The sines of a workgroup's tokens
 // are made once, in LDS, for all of their heads; then the lanes run along the heads, two
 // 16-byte pieces each, whose elements are pairs of each other (interleaved: pairs in
-// themselves).  Where a head does not divide into such pieces the pieces are one element, at a
-// third of the rate.
+// themselves).  Where heads, pairs, strides and addresses are not all whole pieces, the pieces are one
+// element, at a third of the rate (9 heads of 82: 1.7 TB/s; 20 of 80 elements turned: 1.4).
 #include "common.h"
 #include "rotary.h"
 

@@ -56,7 +56,9 @@ class QuantCache:
     scale, which rounds its older tokens again only where their codes fall below 2 ** -6.
 
     All five are advanced in place, on the device.  A count may be set back (to drop drafted
-    tokens, or to 0 to take a row into use again).  Tokens past the capacity are counted but not stored, and
+    tokens, or to 0 to take a row into use again): the scale of the block that it then ends in stays what
+    the dropped tokens made it, and so do the codes of those before them (to go back exactly, keep that
+    block's codes and scales).  Tokens past the capacity are counted but not stored, and
     attention gives NaN for such a row."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "counts", "_layout")
